@@ -351,6 +351,79 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
                     const void* table, int dtype, int M, int H, long long V, void* out,
                     void* zero_out, void* stream);
 
+/*
+ * Paged KV cache and drafted trees (no counterpart in the reference, whose decode
+ * step is projections only; bench/bench_model.py:57-86).  A pool holds `num_pages`
+ * pages of `page_size` rows (a power of two in [8, 1024]); a row is one token's
+ * [Hkv, D] keys (values) of one layer.  Caches are given by their base and the
+ * element strides between pages, rows and heads (multiples of 8; D contiguous),
+ * the same for K and V.  block_table [B, table_width] (row stride table_stride)
+ * names the page of each run of page_size tokens of a request.  The new tokens of
+ * all requests lie behind one another; cu_new [B + 1] says where each begins.
+ *
+ *   ng_paged_plan: the plan of a step from the requests' lengths, in order:
+ *     need[b] = max(0, ceil((cached[b] + new[b]) / page_size) - held[b]) pages, taken from
+ *     free_pages[cursor ..] (cursor: device int or NULL = 0).  A request whose
+ *     pages are not there, or do not fit its table row, is not granted: its
+ *     slots are -1, its kv_lens 0, its table row and held_out as before.
+ *     Outputs: cu_new [B + 1]; per token slots (page * page_size + row),
+ *     positions (cached + depth in its tree; + its place without parents), mask
+ *     [num_tokens, mask_words] (bit j: new token j of the request is an ancestor
+ *     or the token itself); per request kv_lens (cached + new) and held_out
+ *     (pages now held); taken [1] = pages taken.  parents [num_tokens] (may be
+ *     NULL): index of the parent within the request, below the token's own, or
+ *     -1.  num_tokens is the capacity of the per-token outputs; rows past the
+ *     last token get slot -1, position 0, mask 0.  B <= 16384, mask_words <= 64.
+ *     Negative lengths, more tokens than num_tokens, a parent that is not below
+ *     its child, a tree beyond 64 * mask_words nodes: NG_ERR_BAD_INDEX in
+ *     ng_device_status, and nothing is written out of bounds.
+ *   ng_qk_norm_rope_append: rows of qkv [M, (Hq + 2 Hkv) * D] (row stride
+ *     qkv_stride): q and k heads are normalised by their root mean square and
+ *     scaled by q_weight / k_weight [D] (both NULL: not normalised), the first
+ *     rotary_dim values (a multiple of 16, <= D; pairs (i, i + rotary_dim / 2))
+ *     rotated by positions[m] * turns[i] / 2^64 turns, then q -> q_out [M, Hq, D] and k, v ->
+ *     cache row slots[m] (negative: not stored; past the pool: not stored, and
+ *     NG_ERR_BAD_INDEX in ng_device_status).  D 64, 128 or 256.
+ *   ng_tree_attn: out [T, Hq, D] = softmax(scale * q K^T) V of each new token over its
+ *     request's first kv_lens[b] cache rows.  The last n = cu_new[b+1] - cu_new[b] of them are
+ *     the new tokens' own: row i sees them by its mask bits (mask [T, mask_words]
+ *     or NULL: the chain, j <= i) and sees all rows before them.  A row that sees
+ *     nothing gives zeros.  lse [T, Hq] (may be NULL): log of the sum of
+ *     exponentials, -inf for such a row.  D 64 or 128, Hq / Hkv <= 128, scale > 0.
+ *     workspace: ng_tree_attn_workspace_bytes(D) bytes, 256-byte aligned; calls sharing it must
+ *     not overlap on the GPU.  A page outside the pool reads as zeros and sets
+ *     NG_ERR_BAD_INDEX in ng_device_status.
+ *   ng_tree_commit: greedy acceptance.  The path starts at node 0 and goes on to
+ *     the first child c with draft[c] == next[current], at most max_path (<= 512) nodes;
+ *     in each of `layers` caches (stride_layer apart) row before + i becomes row
+ *     before + path[i], before = kv_lens[b] - n.  accepted [B], path [B, max_path] (-1 beyond),
+ *     bonus [B] = next at the path's end (-1 without tokens), kv_out [B] =
+ *     before + accepted (a request without tokens keeps kv_lens). */
+int ng_paged_plan(const int* cached, const int* new_lens, const int* held, int* block_table,
+                  long long table_stride, int table_width, const int* free_pages, int num_free,
+                  const int* cursor, const int* parents, int B, int num_tokens, int page_size,
+                  int mask_words, int* cu_new, int* slots, int* positions, int* kv_lens, int* held_out,
+                  int* taken, long long* mask, void* stream);
+int ng_qk_norm_rope_append(const void* qkv, long long qkv_stride, const void* q_weight,
+                           const void* k_weight, const long long* turns, int rotary_dim,
+                           const int* positions, const int* slots, void* q_out, void* k_cache,
+                           void* v_cache, long long stride_page, long long stride_row,
+                           long long stride_head, int dtype, int M, int Hq, int Hkv, int D,
+                           int num_pages, int page_size, float eps, void* stream);
+size_t ng_tree_attn_workspace_bytes(int D);
+int ng_tree_attn(const void* q, long long q_stride_token, long long q_stride_head, const void* k_cache,
+                 const void* v_cache, long long stride_page, long long stride_row, long long stride_head,
+                 const int* block_table, long long table_stride, int table_width, const int* kv_lens,
+                 const int* cu_new, const long long* mask, int mask_words, void* out, float* lse,
+                 int dtype, int B, int T, int Hq, int Hkv, int D, int num_pages, int page_size,
+                 float scale, void* workspace, size_t workspace_bytes, void* stream);
+int ng_tree_commit(const long long* draft, const int* parents, const long long* next, const int* cu_new,
+                   const int* kv_lens, const int* block_table, long long table_stride, int table_width,
+                   void* k_cache, void* v_cache, long long stride_layer, long long stride_page,
+                   long long stride_row, long long stride_head, int dtype, int B, int T, int layers,
+                   int Hkv, int D, int num_pages, int page_size, int max_path, int* accepted, int* path,
+                   long long* bonus, int* kv_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,8 @@ from .ops import (DECODE_MAX_M, QuantLinear, check_device, dequant, dequantize, 
                   matmul, reference_matmul, set_debug_checks)
 from .decode_model import LLAMA3_8B_MODEL, LLAMA3_70B_MODEL, Llama3Decoder
 from .importers import from_autogptq, to_autogptq
+from .paged import (PagedPlan, TreeCommit, paged_cache, paged_plan, qk_norm_rope_append, rope_turns,
+                    tree_attention, tree_commit)
 from .quant import QuantizedWeight, pack_nibbles, quantize, unpack_nibbles
 
 __all__ = [
@@ -32,5 +34,13 @@ __all__ = [
     "pack_nibbles",
     "quantize",
     "unpack_nibbles",
+    "PagedPlan",
+    "TreeCommit",
+    "paged_cache",
+    "paged_plan",
+    "qk_norm_rope_append",
+    "rope_turns",
+    "tree_attention",
+    "tree_commit",
 ]
 __version__ = "0.1.0"

@@ -18,7 +18,7 @@ NG_DTYPE_F16 = 0
 NG_DTYPE_BF16 = 1
 
 #: Every symbol the header declares, with (restype, argtypes).
-_P, _I = ctypes.c_void_p, ctypes.c_int
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 SIGNATURES = {
     "ng_abi_version": (_I, []),
     "ng_status_string": (ctypes.c_char_p, [_I]),
@@ -53,6 +53,13 @@ SIGNATURES = {
     "ng_gemv_w4a16_allreduce": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P]),
     "ng_lm_head_argmax": (_I, [_P, _P, _I, _I, _I, _I, ctypes.c_longlong, _P, _P, _P]),
     "ng_embed_tokens": (_I, [_P, _P, _P, _P, _I, _I, _I, ctypes.c_longlong, _P, _P, _P]),
+    "ng_paged_plan": (_I, [_P, _P, _P, _P, _L, _I, _P, _I, _P, _P, _I, _I, _I, _I] + [_P] * 8),
+    "ng_qk_norm_rope_append": (_I, [_P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _L, _L] + [_I] * 7 +
+                               [ctypes.c_float, _P]),
+    "ng_tree_attn_workspace_bytes": (ctypes.c_size_t, [_I]),
+    "ng_tree_attn": (_I, [_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _I, _P, _P, _P, _I, _P, _P] + [_I] * 8 +
+                     [ctypes.c_float, _P, ctypes.c_size_t, _P]),
+    "ng_tree_commit": (_I, [_P] * 6 + [_L, _I, _P, _P, _L, _L, _L, _L] + [_I] * 9 + [_P] * 5),
 }
 
 _lib = None

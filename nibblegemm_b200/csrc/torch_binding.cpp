@@ -2,7 +2,7 @@
 // (gemv_w4a16, gemm_w4a16, dequant_w4; arvindcr4/nibblegemm csrc/bindings.cpp)
 // taking tensors, with the argument checks, the output allocation, the device
 // guard, the current-stream lookup and the per-stream workspace cache done in
-// C++ -- a few microseconds per call instead of the tens a Python + ctypes path
+// C++ (and the paged-cache ops of paged.py the same way) -- a few microseconds per call instead of the tens a Python + ctypes path
 // costs.  The kernels are the ones of libnibblegemm_b200.so; this file only
 // marshals.  Argument-check failures raise RuntimeError (TORCH_CHECK), as the
 // reference's do; the library's own status is returned beside the output and
@@ -15,6 +15,7 @@
 #include <optional>
 #include <tuple>
 #include <unordered_map>
+#include <vector>
 
 #include "nibblegemm_b200.h"
 
@@ -135,6 +136,196 @@ std::tuple<torch::Tensor, int64_t> dequant_w4(torch::Tensor Wq, torch::Tensor S,
   return {out, st};
 }
 
+// ---------------------------------------------------------------------------
+// Paged KV cache and drafted trees.
+// ---------------------------------------------------------------------------
+void check_ints(const torch::Tensor& t, const torch::Device& dev, torch::ScalarType type, int64_t dim,
+                const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
+  TORCH_CHECK(t.dim() == dim && t.is_contiguous(), name, " must be a contiguous ", dim, "-D tensor");
+}
+
+// A [.., pages, page_size, heads, D] cache pair: same type, shape and strides, D contiguous.
+void check_caches(const torch::Tensor& K, const torch::Tensor& V, int64_t dim, const torch::Device& dev) {
+  TORCH_CHECK(K.is_cuda() && K.device() == dev && V.device() == dev, "the caches must be on the same CUDA device");
+  dtype_code(K);
+  TORCH_CHECK(K.dim() == dim && V.dim() == dim, "the caches must be ", dim, "-D");
+  TORCH_CHECK(K.sizes() == V.sizes() && K.strides() == V.strides() && K.scalar_type() == V.scalar_type(),
+              "the K and V caches must have the same type, shape and strides");
+  TORCH_CHECK(K.stride(dim - 1) == 1, "the caches' last dimension must be contiguous");
+}
+
+// Row stride of a block table whose rows are contiguous.
+int64_t check_table(const torch::Tensor& t, const torch::Device& dev, int64_t B) {
+  TORCH_CHECK(t.device() == dev && t.scalar_type() == torch::kInt && t.dim() == 2 && t.size(0) == B &&
+                  t.stride(1) == 1 && t.size(1) >= 1,
+              "block_table must be an int32 [requests, blocks] tensor with contiguous rows");
+  return B > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1));
+}
+
+std::tuple<std::vector<std::optional<torch::Tensor>>, int64_t> paged_plan(
+    torch::Tensor cached, torch::Tensor fresh, torch::Tensor held, torch::Tensor table, torch::Tensor free_pages,
+    int64_t page_size, int64_t num_tokens, std::optional<torch::Tensor> parents, int64_t mask_words,
+    std::optional<torch::Tensor> cursor) {
+  TORCH_CHECK(cached.is_cuda(), "all tensors must live on CUDA");
+  const auto dev = cached.device();
+  const int64_t B = cached.size(0);
+  check_ints(cached, dev, torch::kInt, 1, "cached");
+  check_ints(fresh, dev, torch::kInt, 1, "new");
+  check_ints(held, dev, torch::kInt, 1, "held");
+  check_ints(free_pages, dev, torch::kInt, 1, "free_pages");
+  TORCH_CHECK(fresh.size(0) == B && held.size(0) == B, "cached, new and held must have one entry per request");
+  const int64_t stride = check_table(table, dev, B);
+  TORCH_CHECK(num_tokens >= 0 && num_tokens <= (1 << 30), "num_tokens out of range");
+  TORCH_CHECK(mask_words == 0 || parents.has_value(), "a mask needs parents");
+  if (parents.has_value()) {
+    check_ints(*parents, dev, torch::kInt, 1, "parents");
+    TORCH_CHECK(parents->size(0) == num_tokens, "parents must have num_tokens entries");
+  }
+  if (cursor.has_value()) {
+    check_ints(*cursor, dev, torch::kInt, 1, "cursor");
+    TORCH_CHECK(cursor->size(0) == 1, "cursor must have one entry");
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  auto cu = torch::empty({B + 1}, cached.options()), slots = torch::empty({num_tokens}, cached.options()),
+       positions = torch::empty({num_tokens}, cached.options()), kv = torch::empty({B}, cached.options()),
+       held_out = torch::empty({B}, cached.options()), taken = torch::empty({1}, cached.options());
+  std::optional<torch::Tensor> mask;
+  if (mask_words > 0) mask = torch::empty({num_tokens, mask_words}, cached.options().dtype(torch::kLong));
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int st = ng_paged_plan(
+      cached.data_ptr<int>(), fresh.data_ptr<int>(), held.data_ptr<int>(), table.data_ptr<int>(), stride,
+      static_cast<int>(table.size(1)), free_pages.data_ptr<int>(), static_cast<int>(free_pages.size(0)),
+      cursor ? cursor->data_ptr<int>() : nullptr, parents ? parents->data_ptr<int>() : nullptr,
+      static_cast<int>(B), static_cast<int>(num_tokens), static_cast<int>(page_size),
+      static_cast<int>(mask_words), cu.data_ptr<int>(), slots.data_ptr<int>(), positions.data_ptr<int>(),
+      kv.data_ptr<int>(), held_out.data_ptr<int>(), taken.data_ptr<int>(),
+      mask ? reinterpret_cast<long long*>(mask->data_ptr<int64_t>()) : nullptr, stream);
+  return {{cu, slots, positions, kv, held_out, taken, mask}, st};
+}
+
+std::tuple<torch::Tensor, int64_t> qk_norm_rope_append(
+    torch::Tensor qkv, std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight,
+    torch::Tensor turns, torch::Tensor positions, torch::Tensor slots, torch::Tensor K, torch::Tensor V,
+    int64_t q_heads, double eps, std::optional<torch::Tensor> out) {
+  TORCH_CHECK(qkv.is_cuda(), "all tensors must live on CUDA");
+  const auto dev = qkv.device();
+  check_caches(K, V, 4, dev);
+  const int64_t M = qkv.size(0), Hkv = K.size(2), D = K.size(3);
+  TORCH_CHECK(qkv.scalar_type() == K.scalar_type(), "qkv and the caches must have the same type");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (q_heads + 2 * Hkv) * D && qkv.stride(1) == 1,
+              "qkv must be [tokens, (q_heads + 2 kv_heads) * D] with contiguous rows");
+  check_ints(turns, dev, torch::kLong, 1, "turns");
+  check_ints(positions, dev, torch::kInt, 1, "positions");
+  check_ints(slots, dev, torch::kInt, 1, "slots");
+  TORCH_CHECK(positions.size(0) == M && slots.size(0) == M, "positions and slots must have one entry per token");
+  TORCH_CHECK(q_weight.has_value() == k_weight.has_value(), "give both norm weights or neither");
+  for (const auto* w : {&q_weight, &k_weight})
+    if (w->has_value())
+      TORCH_CHECK((*w)->device() == dev && (*w)->scalar_type() == qkv.scalar_type() && (*w)->dim() == 1 &&
+                      (*w)->size(0) == D && (*w)->is_contiguous(),
+                  "a norm weight must be a contiguous [D] tensor of the type of qkv");
+  if (out.has_value())
+    TORCH_CHECK(out->device() == dev && out->scalar_type() == qkv.scalar_type() && out->is_contiguous() &&
+                    out->sizes() == torch::IntArrayRef({M, q_heads, D}),
+                "out must be a contiguous [tokens, q_heads, D] tensor like qkv");
+  const c10::cuda::CUDAGuard guard(dev);
+  auto q = out.has_value() ? *out : torch::empty({M, q_heads, D}, qkv.options());
+  if (M == 0) return {q, 0};
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int st = ng_qk_norm_rope_append(
+      qkv.data_ptr(), M > 1 ? qkv.stride(0) : qkv.size(1), q_weight ? q_weight->data_ptr() : nullptr,
+      k_weight ? k_weight->data_ptr() : nullptr, reinterpret_cast<const long long*>(turns.data_ptr<int64_t>()),
+      static_cast<int>(2 * turns.size(0)), positions.data_ptr<int>(), slots.data_ptr<int>(), q.data_ptr(),
+      K.data_ptr(), V.data_ptr(), K.stride(0), K.stride(1), K.stride(2), dtype_code(qkv), static_cast<int>(M),
+      static_cast<int>(q_heads), static_cast<int>(Hkv), static_cast<int>(D), static_cast<int>(K.size(0)),
+      static_cast<int>(K.size(1)), static_cast<float>(eps), stream);
+  return {q, st};
+}
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, int64_t> tree_attention(
+    torch::Tensor q, torch::Tensor K, torch::Tensor V, torch::Tensor table, torch::Tensor kv_lens,
+    torch::Tensor cu_new, std::optional<torch::Tensor> mask, double scale, bool return_lse,
+    std::optional<torch::Tensor> out) {
+  TORCH_CHECK(q.is_cuda(), "all tensors must live on CUDA");
+  const auto dev = q.device();
+  check_caches(K, V, 4, dev);
+  TORCH_CHECK(q.dim() == 3 && q.scalar_type() == K.scalar_type() && q.size(2) == K.size(3) && q.stride(2) == 1,
+              "q must be [tokens, q_heads, D] of the caches' type with D contiguous");
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), B = kv_lens.size(0);
+  check_ints(kv_lens, dev, torch::kInt, 1, "kv_lens");
+  check_ints(cu_new, dev, torch::kInt, 1, "cu_new");
+  TORCH_CHECK(cu_new.size(0) == B + 1, "cu_new must have one entry more than kv_lens");
+  const int64_t stride = check_table(table, dev, B);
+  if (mask.has_value()) {
+    check_ints(*mask, dev, torch::kLong, 2, "mask");
+    TORCH_CHECK(mask->size(0) == T && mask->size(1) >= 1, "mask must be [tokens, words]");
+  }
+  if (out.has_value())
+    TORCH_CHECK(out->device() == dev && out->scalar_type() == q.scalar_type() && out->is_contiguous() &&
+                    out->sizes() == q.sizes(),
+                "out must be a contiguous tensor like q");
+  const c10::cuda::CUDAGuard guard(dev);
+  auto y = out.has_value() ? *out : torch::empty({T, Hq, D}, q.options());
+  std::optional<torch::Tensor> lse;
+  if (return_lse) lse = torch::empty({T, Hq}, q.options().dtype(torch::kFloat));
+  if (T == 0 || B == 0) return {y, lse, 0};
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  auto ws = workspace(dev, stream, 2, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
+  const int st = ng_tree_attn(
+      q.data_ptr(), q.stride(0), q.stride(1), K.data_ptr(), V.data_ptr(), K.stride(0), K.stride(1), K.stride(2),
+      table.data_ptr<int>(), stride, static_cast<int>(table.size(1)), kv_lens.data_ptr<int>(),
+      cu_new.data_ptr<int>(), mask ? reinterpret_cast<const long long*>(mask->data_ptr<int64_t>()) : nullptr,
+      mask ? static_cast<int>(mask->size(1)) : 0, y.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
+      dtype_code(q), static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(K.size(2)),
+      static_cast<int>(D), static_cast<int>(K.size(0)), static_cast<int>(K.size(1)), static_cast<float>(scale),
+      ws.data_ptr(), static_cast<size_t>(ws.numel()), stream);
+  return {y, lse, st};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, int64_t> tree_commit(
+    torch::Tensor draft, torch::Tensor parents, torch::Tensor next, torch::Tensor cu_new, torch::Tensor kv_lens,
+    torch::Tensor table, torch::Tensor K, torch::Tensor V, int64_t max_path) {
+  TORCH_CHECK(draft.is_cuda(), "all tensors must live on CUDA");
+  const auto dev = draft.device();
+  TORCH_CHECK(K.dim() == 4 || K.dim() == 5, "the caches must be [layers, pages, page_size, heads, D] or one layer of it");
+  const int64_t o = K.dim() - 4;
+  check_caches(K, V, 4 + o, dev);
+  check_ints(draft, dev, torch::kLong, 1, "draft");
+  check_ints(next, dev, torch::kLong, 1, "next");
+  check_ints(parents, dev, torch::kInt, 1, "parents");
+  check_ints(cu_new, dev, torch::kInt, 1, "cu_new");
+  check_ints(kv_lens, dev, torch::kInt, 1, "kv_lens");
+  const int64_t B = kv_lens.size(0), T = draft.size(0);
+  TORCH_CHECK(next.size(0) == T && parents.size(0) == T, "draft, parents and next must have one entry per token");
+  TORCH_CHECK(cu_new.size(0) == B + 1, "cu_new must have one entry more than kv_lens");
+  TORCH_CHECK(max_path >= 1 && max_path <= 512, "max_path must be 1..512");
+  const int64_t stride = check_table(table, dev, B);
+  const c10::cuda::CUDAGuard guard(dev);
+  auto accepted = torch::empty({B}, kv_lens.options()), path = torch::empty({B, max_path}, kv_lens.options()),
+       bonus = torch::empty({B}, draft.options()), kv_out = torch::empty({B}, kv_lens.options());
+  if (B == 0) return {accepted, path, bonus, kv_out, 0};
+  if (T == 0) {
+    accepted.zero_();
+    path.fill_(-1);
+    bonus.fill_(-1);
+    kv_out.copy_(kv_lens);
+    return {accepted, path, bonus, kv_out, 0};
+  }
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  auto* ll = +[](torch::Tensor& t) { return reinterpret_cast<long long*>(t.data_ptr<int64_t>()); };
+  const int st = ng_tree_commit(
+      ll(draft), parents.data_ptr<int>(), ll(next), cu_new.data_ptr<int>(), kv_lens.data_ptr<int>(),
+      table.data_ptr<int>(), stride, static_cast<int>(table.size(1)), K.data_ptr(), V.data_ptr(),
+      o ? K.stride(0) : 0, K.stride(o), K.stride(o + 1), K.stride(o + 2), dtype_code(K), static_cast<int>(B),
+      static_cast<int>(T), o ? static_cast<int>(K.size(0)) : 1, static_cast<int>(K.size(o + 2)),
+      static_cast<int>(K.size(o + 3)), static_cast<int>(K.size(o)), static_cast<int>(K.size(o + 1)),
+      static_cast<int>(max_path), accepted.data_ptr<int>(), path.data_ptr<int>(), ll(bonus),
+      kv_out.data_ptr<int>(), stream);
+  return {accepted, path, bonus, kv_out, st};
+}
+
 // The cached workspace a call on (device, stream) uses (for inspection).
 torch::Tensor workspace_for(int64_t device_index, int64_t stream, int64_t kind, int64_t need) {
   return workspace(torch::Device(torch::kCUDA, static_cast<c10::DeviceIndex>(device_index)),
@@ -150,8 +341,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_w4a16", &gemm_w4a16, "Prefill-regime W4A16 GEMM (tcgen05).", py::arg("X"), py::arg("Wq"),
         py::arg("S"), py::arg("group_size"), py::arg("version") = 6, py::arg("tile_tokens") = 0,
         py::arg("out") = py::none());
-  m.def("workspace", &workspace_for, "The zero-initialised workspace of (device, stream); kind 0 = GEMV, 1 = GEMM.",
+  m.def("workspace", &workspace_for, "The zero-initialised workspace of (device, stream); kind 0 = GEMV, 1 = GEMM, 2 = tree attention.",
         py::arg("device_index"), py::arg("stream"), py::arg("kind"), py::arg("need"));
+  m.def("paged_plan", &paged_plan);
+  m.def("qk_norm_rope_append", &qk_norm_rope_append);
+  m.def("tree_attention", &tree_attention);
+  m.def("tree_commit", &tree_commit);
   m.def("dequant_w4", &dequant_w4, "Packed INT4 to dense fp16 / bf16.", py::arg("Wq"), py::arg("S"),
         py::arg("group_size"), py::arg("fast") = true, py::arg("out_dtype") = py::none());
 }

@@ -1,0 +1,146 @@
+// Greedy acceptance of a drafted tree and the move of its cache rows.
+//   path_0 = 0 (the request's last known token, the root);
+//   path_{i+1} = the first child c of path_i with draft[c] == next[path_i];
+//   the walk ends at a node without such a child, or at max_path nodes.
+// Then, for every layer, cache row (before + i) <- row (before + path_i), with
+// before = kv - n the rows in front of the tree: the kept nodes become the
+// context's last rows and the rest is free to be written over.  path is
+// increasing, so row i is never the source of a later move once written
+// (path_j > path_i >= i for j > i): copying in the order of i needs no buffer.
+//
+// One CTA per (request, layer, share of the heads); every CTA repeats the walk (a
+// few steps over the tree's nodes, one warp, children found by ballot) rather
+// than wait for another kernel.  A thread owns 16-byte columns of a row and
+// moves them path step by path step, so moves of one column stay in order.
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+namespace ngb {
+namespace {
+
+constexpr int kCommitThreads = 128;
+constexpr int kCommitMaxPath = 512;
+
+struct CommitArgs {
+  const long long* draft;
+  const int* parents;
+  const long long* next;
+  const int* cu;
+  const int* kv;
+  const int* table;
+  long long table_stride;
+  int table_width;
+  uint4* k_cache;
+  uint4* v_cache;
+  long long s_layer, s_page, s_row, s_head;  // in 16-byte units
+  int B, T, Hkv, vecs, num_pages, page_shift, max_path;
+  int* accepted;
+  int* path;
+  long long* bonus;
+  int* kv_out;
+  unsigned int* err;
+};
+
+__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs p) {
+  __shared__ int path[kCommitMaxPath];
+  __shared__ int count_s;
+  pdl_launch_next();
+  pdl_wait_previous();
+  const int b = blockIdx.x, layer = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int first = min(max(p.cu[b], 0), p.T), end = min(max(p.cu[b + 1], first), p.T);
+  const int n = end - first;
+  const int kv = p.kv[b];
+  if (tid < 32) {
+    int count = 0;
+    if (n > 0 && kv >= n) {
+      int cur = 0;
+      for (;;) {
+        if (lane == 0) path[count] = cur;
+        ++count;
+        if (count >= p.max_path) break;
+        const long long want = p.next[first + cur];
+        int found = -1;
+        for (int c0 = cur + 1; c0 < n && found < 0; c0 += 32) {  // children come after their parent
+          const int c = c0 + lane;
+          const bool hit = c < n && p.parents[first + c] == cur && p.draft[first + c] == want;
+          const unsigned vote = __ballot_sync(0xffffffffu, hit);
+          if (vote) found = c0 + __ffs(vote) - 1;
+        }
+        if (found < 0) break;
+        cur = found;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) count_s = count;
+    if (layer == 0 && blockIdx.z == 0) {
+      if (lane == 0) {
+        p.accepted[b] = count;
+        p.bonus[b] = count ? p.next[first + path[count - 1]] : -1;
+        p.kv_out[b] = count ? kv - n + count : kv;
+        if (n > 0 && kv < n && kv != 0) atomicOr(p.err, kErrBadIndex);
+      }
+      for (int i = lane; i < p.max_path; i += 32)
+        p.path[static_cast<size_t>(b) * p.max_path + i] = i < count ? path[i] : -1;
+    }
+  }
+  __syncthreads();
+  const int count = count_s, before = kv - n;
+  const int ps_mask = (1 << p.page_shift) - 1;
+  const int* row = p.table + static_cast<size_t>(b) * p.table_stride;
+  auto offset = [&](int at) -> long long {  // 16-byte units of cache row `at`, or -1
+    const int blk = at >> p.page_shift;
+    const int page = blk < p.table_width ? row[blk] : -1;
+    if (page < 0 || page >= p.num_pages) return -1;
+    return page * p.s_page + (at & ps_mask) * p.s_row;
+  };
+  const int columns = p.Hkv * p.vecs;
+  const size_t base = static_cast<size_t>(layer) * p.s_layer;
+  for (int col = blockIdx.z * kCommitThreads + tid; col < columns; col += gridDim.z * kCommitThreads) {
+    const size_t at = base + static_cast<size_t>(col / p.vecs) * p.s_head + col % p.vecs;
+    for (int i = 0; i < count; ++i) {
+      if (path[i] == i) continue;
+      const long long from = offset(before + path[i]), to = offset(before + i);
+      if (from < 0 || to < 0) {
+        atomicOr(p.err, kErrBadIndex);
+        continue;
+      }
+      p.k_cache[at + to] = p.k_cache[at + from];
+      p.v_cache[at + to] = p.v_cache[at + from];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace ngb
+
+extern "C" int ng_tree_commit(const long long* draft, const int* parents, const long long* next,
+                              const int* cu_new, const int* kv_lens, const int* block_table,
+                              long long table_stride, int table_width, void* k_cache, void* v_cache,
+                              long long stride_layer, long long stride_page, long long stride_row,
+                              long long stride_head, int dtype, int B, int T, int layers, int Hkv, int D,
+                              int num_pages, int page_size, int max_path, int* accepted, int* path,
+                              long long* bonus, int* kv_out, void* stream) {
+  using namespace ngb;
+  if (!draft || !parents || !next || !cu_new || !kv_lens || !block_table || !k_cache || !v_cache || !accepted ||
+      !path || !bonus || !kv_out)
+    return NG_ERR_NULL_POINTER;
+  if (!act_dtype_ok(dtype)) return NG_ERR_BAD_DTYPE;
+  if (B < 1 || T < 1 || layers < 1 || layers > 65535 || Hkv < 1 || D < 8 || D % 8 || num_pages < 1 ||
+      table_width < 1 || table_stride < table_width || !page_size_ok(page_size))
+    return NG_ERR_BAD_SHAPE;
+  const CacheStrides cs{stride_page, stride_row, stride_head};
+  if (!cache_strides_ok(cs) || stride_layer % 8 || stride_layer < 0) return NG_ERR_BAD_SHAPE;
+  if (max_path < 1 || max_path > kCommitMaxPath) return NG_ERR_BAD_ARGUMENT;
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return NG_ERR_MISALIGNED;
+  DeviceInfo dev;
+  if (int st = current_device_info(&dev)) return st;
+  const CommitArgs a{draft, parents, next, cu_new, kv_lens, block_table, table_stride, table_width,
+                     static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), stride_layer / 8,
+                     stride_page / 8, stride_row / 8, stride_head / 8, B, T, Hkv, D / 8, num_pages,
+                     log2_of(page_size), max_path, accepted, path, bonus, kv_out, dev.err};
+  const int shares = std::max(1, (Hkv * (D / 8) + kCommitThreads - 1) / kCommitThreads);
+  return launch_chained(tree_commit_kernel, dim3(B, layers, std::min(shares, 64)), dim3(kCommitThreads), 0,
+                        static_cast<cudaStream_t>(stream), a);
+}
