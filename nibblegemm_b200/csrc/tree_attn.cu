@@ -1,15 +1,110 @@
-// Attention of drafted trees, chains or single tokens over a paged KV cache.
+// Attention of drafted trees, chains or single tokens over a paged KV cache:
+//   out_i = sum_j p_ij v_j,  p_ij = exp(s_ij - m_i) / sum_j exp(s_ij - m_i),
+//   s_ij = scale q_i . k_j over the keys j that row i sees:
+// all rows of the cache in front of the request's new tokens, and of the new
+// tokens' own rows those that its mask names (or j <= i without a mask).
+//
+// The query heads that share a KV head are rows of one tile: row r of a tile is
+// token r / G, head r % G (G = Hq / Hkv), so K and V are read once for all of them
+// and a tile of 128 rows holds 128 / G tokens.  A work item is (request, KV head,
+// two tiles of tokens); its keys come in tiles of 128.
+//
+// One persistent CTA per SM, warp-specialised:
+//   warps 0-3, 4-7  softmax of stream 0 and stream 1, one thread per row
+//   warp 8          TMA: the pages of a K or V tile into a ring of stages, one lane per
+//                   page and 64-value half, 128-byte swizzle
+//   warp 9          tcgen05.mma: S_s = Q_s K^T (128 x 128, both operands from shared
+//                   memory), O_s += P_s V (P_s from tensor memory)
+//   warp 10         tensor-memory allocation; rows of V that no MMA may see (below)
+//   warp 11         walks this CTA's share of the work and hands out its items
+// The two streams hide each other's softmax: while one is in its exponentials the
+// tensor core works for the other.  With two tiles of tokens both streams go
+// through every key tile (which is loaded once); with one tile they take the even
+// and the odd key tiles, each with a softmax state of its own, and stream 0 joins
+// the two at the end.  Tensor memory: S_0, S_1 (128 columns each; P_s is written over S_s), O_0,
+// O_1 (D each).
+//
+// Work is split evenly over the CTAs: every CTA adds up the key tiles of all items
+// (from the lengths, on the GPU; an item counts one more for its fixed cost) and
+// takes its share of the line, which may begin and end inside an item.  An item
+// that lies in several CTAs is written as unnormalised fp32 partials with their
+// maxima and sums, which a second small kernel joins in CTA order.
+//
+// The running maximum is only raised (and O rescaled) when it grows by more than
+// 8 in base 2: the probabilities then stay below 2^8, the sums are fp32, and
+// nearly all tiles leave O alone.  S, maxima, sums and O are fp32; P is
+// rounded to the activation type, as the tensor core takes no other operand.
+//
+// Masked keys contribute nothing, whatever they hold: masked scores are replaced,
+// not added to, and because 0 * inf is not 0 the rows of V beyond the request's
+// end are zeroed in shared memory, and values that are not finite in rows that
+// some query does not see are zeroed there and added back, in the epilogue, to the
+// rows that do see them.  Only tiles that hold such keys pay for this.
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <mutex>
 
 #include "paged_common.cuh"
+#include "sm100_primitives.cuh"
 
 namespace ngb {
 namespace {
 
+constexpr int kTile = 128;         // rows of a query tile, keys of a key tile
+constexpr int kAttnThreads = 384;  // 12 warps
+constexpr int kRowsMax = 2 * kTile;
+constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
+constexpr int kBadSlots = 8;
+constexpr int kItems = 4;          // work items handed out ahead
+
+// A work item as one CTA sees it.
+struct alignas(16) Item {
+  int b, h, i0, ntok;    // request, KV head, tokens [i0, i0 + ntok) of the request
+  int first, ctx, kv;    // the request's first token row, rows before its new tokens, all rows
+  int need, full;        // keys that the item's tokens need; leading ones that all of them see
+  int nt, lo, hi;        // key tiles of the item; this CTA's are [lo, hi); none: the end of the work
+  int two;               // two tiles of tokens
+  int pad[3];
+};
+
+template <int D>
+struct Shape {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kTile * D * 2;           // a Q, K or V tile
+  static constexpr int kHalfBytes = kTile * 128;             // its 64-value half
+  static constexpr int kStages = D == 128 ? 5 : 10;          // ring: 160 KB
+  static constexpr int kSmem = (2 + kStages) * kTileBytes;
+  // One partial: kRowsMax rows of D values, maxima, sums.
+  static constexpr size_t kPartFloats = static_cast<size_t>(kRowsMax) * (D + 2);
+};
+
+struct alignas(16) Shared {
+  uint64_t full[10], empty[10], vissued[10], vclean[10];
+  uint64_t qfull[2], sfull[2], pfull[2], ofull[2];
+  uint64_t ml1, o1read;
+  uint64_t item_full[kItems], item_empty[kItems];
+  Item items[kItems];
+  long long warp_sum[12];
+  long long start_u;
+  int start_b, start_off;
+  uint32_t tmem;
+  int abort;
+  int bad[kBadSlots];
+  float m1[kTile], l1[kTile];
+};
+
+// What the joining kernel needs to know of a CTA.
+struct Meta {
+  int tail;       // an item begins in this CTA and goes on in the next: its partial is slot 1
+  int head_ends;  // the item of slot 0 ends in this CTA
+  int token, ntok, head;  // first token row, tokens and KV head of the slot 1 item
+  int pad[3];
+};
+
 struct TreeAttnArgs {
   const uint16_t* q;
   long long q_token, q_head;
-  const uint16_t* k;
   const uint16_t* v;
   CacheStrides cs;
   const int* table;
@@ -21,83 +116,879 @@ struct TreeAttnArgs {
   int mask_words;
   uint16_t* out;
   float* lse;
-  int B, T, Hq, Hkv, num_pages, page_shift;
-  float scale;
+  int B, T, Hq, Hkv, G, tok_tile, num_pages, page_shift, min_units;
+  float scale_log2;
+  float* part;
+  Meta* meta;
   unsigned int* err;
 };
 
-// One warp per (token, query head): keys one at a time, online softmax.
+// ---------------------------------------------------------------------------
+// PTX used here only
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc].
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 32 consecutive columns.
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float* f) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(f);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
+// V tile as the MMA's B operand, N (the D values) contiguous: rows of 64 values
+// (128 bytes, 128-byte swizzle), 8 keys per 1024-byte atom.  Stride offset: atoms
+// along the keys, 1024 B; leading offset: the next 64 values, one half on.
+__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t addr, uint32_t half_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(half_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// Bounded wait, one lane or a whole warp; false once the CTA has given up.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, err, abort);
+}
+
+// ---------------------------------------------------------------------------
+// The line of work
+// ---------------------------------------------------------------------------
+struct Request {
+  int first, n, kv, ctx;
+};
+
+__device__ __forceinline__ Request load_request(const TreeAttnArgs& p, int b) {
+  Request r;
+  r.first = min(max(p.cu[b], 0), p.T);
+  r.n = min(max(p.cu[b + 1], r.first), p.T) - r.first;
+  const long long most = static_cast<long long>(p.table_width) << p.page_shift;
+  r.kv = max(p.kv_lens[b], 0);
+  if (r.kv > most) {  // more rows than its table names
+    atomicOr(p.err, kErrBadIndex);
+    r.kv = static_cast<int>(most);
+  }
+  r.ctx = max(0, r.kv - r.n);
+  return r;
+}
+
+// Keys that the tokens [i0, i1) need, and the leading ones that all of them see.
+__device__ __forceinline__ int keys_needed(const TreeAttnArgs& p, const Request& r, int i1) {
+  return p.mask ? r.kv : min(r.kv, r.ctx + i1);
+}
+__device__ __forceinline__ int keys_full(const TreeAttnArgs& p, const Request& r, int i0) {
+  return p.mask ? r.ctx : min(r.kv, r.ctx + i0 + 1);
+}
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
+
+// Units of one KV head of a request: its tiles, and one for each item.
+__device__ __forceinline__ long long head_units(const TreeAttnArgs& p, const Request& r) {
+  const int step = 2 * p.tok_tile;
+  if (p.mask) return static_cast<long long>((r.n + step - 1) / step) * (tiles_of(r.kv) + 1);
+  long long u = 0;
+  for (int i0 = 0; i0 < r.n; i0 += step) u += tiles_of(keys_needed(p, r, min(r.n, i0 + step))) + 1;
+  return u;
+}
+
+struct Walk {
+  long long u, u1;
+  int b, h, i0;
+  int off;
+  Request r;
+
+  __device__ __forceinline__ bool next(const TreeAttnArgs& p, Item& it) {
+    const int step = 2 * p.tok_tile;
+    while (u < u1 && b < p.B) {
+      if (r.n == 0) {
+        if (++b < p.B) r = load_request(p, b);
+        continue;
+      }
+      const int i1 = min(r.n, i0 + step);
+      const int need = keys_needed(p, r, i1);
+      const int nt = tiles_of(need);
+      const int take = static_cast<int>(min(static_cast<long long>(nt + 1 - off), u1 - u));
+      it.b = b, it.h = h, it.i0 = i0, it.ntok = i1 - i0;
+      it.first = r.first, it.ctx = r.ctx, it.kv = r.kv, it.need = need, it.full = keys_full(p, r, i0);
+      it.nt = nt, it.lo = max(0, off - 1), it.hi = off + take - 1;
+      it.two = it.ntok > p.tok_tile;
+      u += take;
+      off += take;
+      if (off == nt + 1) {
+        off = 0;
+        i0 += step;
+        if (i0 >= r.n) {
+          i0 = 0;
+          if (++h == p.Hkv) {
+            h = 0;
+            if (++b < p.B) r = load_request(p, b);
+          }
+        }
+      }
+      if (it.hi > it.lo) return true;
+    }
+    return false;
+  }
+};
+
+// Place of key tile j (of n) in the order in which the tiles are loaded: with two
+// query tiles K0 V0 K1 V1 ..., with one K0 K1 V0 K2 V1 ... (the order of the MMAs).
+__device__ __forceinline__ int k_place(bool two, int j) { return two ? 2 * j : (j ? 2 * j - 1 : 0); }
+__device__ __forceinline__ int v_place(bool two, int j, int n) {
+  return two ? 2 * j + 1 : (j == n - 1 ? 2 * n - 1 : 2 * j + 2);
+}
+
+// 32 bits of token row `row`'s mask from bit `at` on (which may be negative).
+__device__ __forceinline__ uint32_t mask_window(const TreeAttnArgs& p, int row, int at) {
+  if (at <= -32) return 0;
+  const unsigned long long* m = p.mask + static_cast<size_t>(row) * p.mask_words;
+  auto word = [&](int i) { return i < p.mask_words ? m[i] : 0ull; };
+  if (at < 0) return static_cast<uint32_t>(word(0) << -at);
+  const int w = at >> 6, s = at & 63;
+  unsigned long long v = word(w) >> s;
+  if (s > 32) v |= word(w + 1) << (64 - s);
+  return static_cast<uint32_t>(v);
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Which of the 32 keys from `key` on token i of the item's request sees.
+__device__ __forceinline__ uint32_t visible(const TreeAttnArgs& p, const Item& it, int i, int key) {
+  if (!p.mask) return low_bits(min(it.kv, it.ctx + i + 1) - key);
+  return (low_bits(it.ctx - key) | mask_window(p, it.first + i, key - it.ctx)) & low_bits(it.kv - key);
+}
+
+// ---------------------------------------------------------------------------
+// Main kernel
+// ---------------------------------------------------------------------------
 template <bool BF16, int D>
-__global__ void __launch_bounds__(128) tree_attn_simple(const TreeAttnArgs p) {
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                     const __grid_constant__ TreeAttnArgs p) {
+  using Sh = Shape<D>;
+  constexpr int kStages = Sh::kStages;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                         ~static_cast<uintptr_t>(1023));
+  unsigned char* ring = smem + 2 * Sh::kTileBytes;  // after Q_0, Q_1
+  Shared* sh = reinterpret_cast<Shared*>(smem + Sh::kSmem);
+  volatile int* abort = &sh->abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+      mbar_init(&sh->vissued[s], 1);
+      mbar_init(&sh->vclean[s], 1);
+    }
+    for (int s = 0; s < kItems; ++s) {
+      mbar_init(&sh->item_full[s], 1);
+      mbar_init(&sh->item_empty[s], 11);  // TMA, MMA, V rows, 8 softmax warps
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh->qfull[s], 4);
+      mbar_init(&sh->sfull[s], 1);
+      mbar_init(&sh->pfull[s], 4);
+      mbar_init(&sh->ofull[s], 1);
+    }
+    mbar_init(&sh->ml1, 4);
+    mbar_init(&sh->o1read, 4);
+    sh->abort = 0;
+    sh->start_b = p.B;
+    for (int i = 0; i < kBadSlots; ++i) sh->bad[i] = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 10) tmem_alloc(&sh->tmem, 512);
+  pdl_launch_next();
+  pdl_wait_previous();
+
+  // ---- this CTA's share of the line
+  const int per = (p.B + kAttnThreads - 1) / kAttnThreads;
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += head_units(p, load_request(p, b)) * p.Hkv;
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sh->warp_sum[warp] = inc;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  long long before = inc - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnThreads / 32; ++w) {
+    if (w < warp) before += sh->warp_sum[w];
+    total += sh->warp_sum[w];
+  }
+  // Shares of at least min_units: the last CTAs stay idle when there is little work.
+  const long long ctas = min(static_cast<long long>(gridDim.x), max(1ll, total / p.min_units));
+  const long long u0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+  const long long u1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+  if (u0 < u1 && before <= u0 && u0 < before + mine) {
+    long long at = before;
+    for (int b = b0; b < b1; ++b) {
+      const long long units = head_units(p, load_request(p, b)) * p.Hkv;
+      if (u0 < at + units) {
+        sh->start_b = b;
+        sh->start_u = u0 - at;
+        break;
+      }
+      at += units;
+    }
+  }
+  // rows beyond the last request's tokens see nothing
+  for (long long i = static_cast<long long>(blockIdx.x) * kAttnThreads + tid +
+                     static_cast<long long>(min(max(p.cu[p.B], 0), p.T)) * p.Hq * (D / 8);
+       i < static_cast<long long>(p.T) * p.Hq * (D / 8); i += static_cast<long long>(gridDim.x) * kAttnThreads) {
+    reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
+    if (p.lse && i % (D / 8) == 0) p.lse[i / (D / 8)] = -INFINITY;
+  }
+  __syncthreads();
+  const uint32_t tmem = sh->tmem;
+
+  // The item that is k-th in this CTA: waits for it; false when there is none (or
+  // the CTA has given up).  done(k) after its last use, one lane of a warp.
+  auto item_at = [&](int k) -> const Item& { return sh->items[k % kItems]; };
+  auto next_item = [&](int k) {
+    return wait_bar(&sh->item_full[k % kItems], (k / kItems) & 1, p.err, abort) && item_at(k).hi > item_at(k).lo;
+  };
+  auto done = [&](int k) { mbar_arrive(&sh->item_empty[k % kItems]); };
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    const int shift = min(p.page_shift, 7);         // rows of a piece: a page, or a whole tile of one
+    const int pieces = kTile >> shift;
+    const int piece = lane % pieces, half = lane / pieces;
+    const uint32_t piece_bytes = 128u << shift;
+    const uint32_t offset = half * Sh::kHalfBytes + piece * piece_bytes;
+    const int page_mask = (1 << p.page_shift) - 1;
+    uint32_t it_count = 0;
+    bool ok = true;
+    for (int k = 0; ok && __all_sync(0xffffffffu, next_item(k)); ++k) {
+      const Item it = item_at(k);
+      __syncwarp();
+      if (lane == 0) done(k);
+      const int n = it.hi - it.lo;
+      const int* row = p.table + static_cast<long long>(it.b) * p.table_stride;
+      auto active_at = [&](int j) {
+        return half < Sh::kHalves && (it.lo + j) * kTile + (piece << shift) < it.need;
+      };
+      auto page_at = [&](int j) -> int {
+        if (j >= n || !active_at(j)) return 0;
+        return row[((it.lo + j) * kTile + (piece << shift)) >> p.page_shift];
+      };
+      auto load = [&](bool is_v, int j, int page) {
+        const uint32_t s = it_count % kStages, ph = (it_count / kStages) & 1;
+        ++it_count;
+        if (!__all_sync(0xffffffffu, wait_bar(&sh->empty[s], ph ^ 1, p.err, abort))) return false;
+        const bool active = active_at(j);
+        const unsigned votes = __ballot_sync(0xffffffffu, active);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->full[s], __popc(votes) * piece_bytes);
+          // From here on the parity of full[s] means this use to the V-row warp, which
+          // only looks at some uses and could take another for it.
+          if (is_v && (it.lo + j + 1) * kTile > it.full) mbar_arrive(&sh->vissued[s]);
+        }
+        __syncwarp();
+        if (active) {
+          if (page < 0 || page >= p.num_pages) {  // outside the pool: the load fills zeros
+            atomicOr(p.err, kErrBadIndex);
+            page = p.num_pages;
+          }
+          const int r = ((it.lo + j) * kTile + (piece << shift)) & page_mask;
+          tma_load_4d(smem_u32(ring + s * Sh::kTileBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[s],
+                      half * 64, r, it.h, page);
+        }
+        return true;
+      };
+      const int lag = it.two ? 0 : 1;
+      int pg = page_at(0), pg_prev = 0;
+      for (int j = 0; ok && j < n + lag; ++j) {
+        const int pg_next = page_at(j + 1);
+        if (j < n) ok = load(false, j, pg);
+        if (ok && j >= lag) ok = load(true, j - lag, lag ? pg_prev : pg);
+        pg_prev = pg;
+        pg = pg_next;
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kTile);
+      constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
+      uint32_t base = 0;       // ring places used by earlier items
+      uint32_t clean_ph = 0;   // per stage: parity of its next cleaned use
+      uint32_t q_ph = 0, p_ph = 0;  // parities, bit s
+      bool ok = true;
+      for (int k = 0; ok && next_item(k); ++k) {
+        const Item& it = item_at(k);
+        const int n = it.hi - it.lo, lo = it.lo, full = it.full;
+        const bool two = it.two;
+        done(k);
+        const int n0 = two ? n : (n + 1) / 2, n1 = two ? n : n / 2;
+        auto scores = [&](int s, int i) {  // S_s = Q_s K^T of the stream's i-th tile
+          const int j = two ? i : 2 * i + s;
+          const uint32_t pl = base + k_place(two, j);
+          const uint32_t st = pl % kStages;
+          if (!wait_bar(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          tc_fence_after();
+          const uint32_t qa = smem_u32(smem + s * Sh::kTileBytes), ka = smem_u32(ring + st * Sh::kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t o = (kk >> 2) * Sh::kHalfBytes + (kk & 3) * 32;
+            umma_f16(tmem + s * kTile, sw128_kmajor_desc(qa + o), sw128_kmajor_desc(ka + o), idesc_s, kk != 0);
+          }
+          umma_commit(&sh->sfull[s]);
+          if (!two || s == 1) umma_commit(&sh->empty[st]);
+          return true;
+        };
+        auto values = [&](int s, int i) {  // O_s += P_s V
+          const int j = two ? i : 2 * i + s;
+          const uint32_t pl = base + v_place(two, j, n);
+          const uint32_t st = pl % kStages;
+          if (!wait_bar(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          if ((lo + j + 1) * kTile > full) {
+            if (!wait_bar(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort)) return false;
+            if (!two || s == 1) clean_ph ^= 1u << st;
+          }
+          tc_fence_after();
+          const uint32_t va = smem_u32(ring + st * Sh::kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            umma_f16_ts(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8,
+                        sw128_nmajor_desc(va + kk * 2048, Sh::kHalfBytes), idesc_o, (i | kk) != 0);
+          if (!two || s == 1) umma_commit(&sh->empty[st]);
+          if (i == (s ? n1 : n0) - 1) umma_commit(&sh->ofull[s]);
+          return true;
+        };
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (ok && (s ? n1 : n0) > 0) {
+            ok = wait_bar(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
+            q_ph ^= 1u << s;
+            ok = ok && scores(s, 0);
+          }
+        for (int i = 0; ok && i < n0; ++i) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int mine_n = s ? n1 : n0;
+            if (ok && i < mine_n) {
+              ok = wait_bar(&sh->pfull[s], (p_ph >> s) & 1, p.err, abort);
+              p_ph ^= 1u << s;
+              ok = ok && values(s, i);
+              if (ok && i + 1 < mine_n) ok = scores(s, i + 1);
+            }
+          }
+        }
+        base += 2 * n;
+      }
+    }
+  } else if (warp == 11) {
+    // ------------------------------------------------------------ the items
+    if (lane == 0) {
+      Walk walk;
+      walk.b = sh->start_b, walk.h = 0, walk.i0 = 0, walk.off = 0;
+      walk.u = u0, walk.u1 = u1;
+      if (walk.b < p.B) {
+        walk.r = load_request(p, walk.b);
+        const int step = 2 * p.tok_tile;
+        const long long per_head = head_units(p, walk.r);
+        long long o = sh->start_u;
+        walk.h = static_cast<int>(o / per_head);
+        o -= walk.h * per_head;
+        for (;;) {
+          const int units = tiles_of(keys_needed(p, walk.r, min(walk.r.n, walk.i0 + step))) + 1;
+          if (o < units) break;
+          o -= units;
+          walk.i0 += step;
+        }
+        walk.off = static_cast<int>(o);
+      }
+      for (int k = 0;; ++k) {
+        if (!wait_bar(&sh->item_empty[k % kItems], ((k / kItems) & 1) ^ 1, p.err, abort)) break;
+        Item it;
+        const bool more = walk.next(p, it);
+        if (!more) it.lo = it.hi = 0;
+        sh->items[k % kItems] = it;
+        mbar_arrive(&sh->item_full[k % kItems]);
+        if (!more) break;
+      }
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ V rows that no MMA may see
+    uint32_t base = 0, issued_ph = 0;
+    bool ok = true;
+    for (int k = 0; ok && __all_sync(0xffffffffu, next_item(k)); ++k) {
+      const Item it = item_at(k);
+      __syncwarp();
+      if (lane == 0) done(k);
+      const int n = it.hi - it.lo, seq = k + 1;
+      for (int j = 0; ok && j < n; ++j) {
+        const int key0 = (it.lo + j) * kTile;
+        if (key0 + kTile <= it.full) continue;
+        const uint32_t pl = base + v_place(it.two, j, n);
+        const uint32_t st = pl % kStages;
+        ok = __all_sync(0xffffffffu, wait_bar(&sh->vissued[st], (issued_ph >> st) & 1, p.err, abort) &&
+                                         wait_bar(&sh->full[st], (pl / kStages) & 1, p.err, abort));
+        if (!ok) break;
+        issued_ph ^= 1u << st;
+        unsigned char* tile = ring + st * Sh::kTileBytes;
+        bool bad = false;
+        for (int r = lane; r < kTile; r += 32) {
+          const int key = key0 + r;
+          if (key < it.full) continue;
+          const bool beyond = key >= it.need;
+#pragma unroll
+          for (int hf = 0; hf < Sh::kHalves; ++hf) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kHalfBytes + r * 128 + (((c + lane) & 7) << 4));
+              if (beyond) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 v = *at;
+              constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+              auto infinite = [&](uint32_t w) { return ((w & kExp) + kOne) & 0x80008000u; };
+              if (infinite(v.x) | infinite(v.y) | infinite(v.z) | infinite(v.w)) {
+                auto clear = [&](uint32_t w) {
+                  const uint32_t f = infinite(w);
+                  return w & ~((f & 0x8000u ? 0xFFFFu : 0u) | (f & 0x80000000u ? 0xFFFF0000u : 0u));
+                };
+                *at = make_uint4(clear(v.x), clear(v.y), clear(v.z), clear(v.w));
+                bad = true;
+              }
+            }
+          }
+        }
+        if (bad) sh->bad[seq % kBadSlots] = seq;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->vclean[st]);
+      }
+      base += 2 * n;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, one thread per row
+    const int s = warp >> 2;             // stream
+    const int row = tid & (kTile - 1);   // row of the tile
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + s * kTile + lanes, to = tmem + 2 * kTile + s * D + lanes;
+    unsigned char* qs = smem + s * Sh::kTileBytes;
+    uint32_t s_ph = 0, o_ph = 0, o1_ph = 0, b_ph = 0;  // parities: S, O, O of stream 1 (kept by stream 0), joins
+    bool o1_pending = false;                        // stream 1: stream 0 has yet to read O_1
+    bool ok = true;
+    const int rt = row / p.G, rg = row - rt * p.G;
+
+    // Q rows of this stream's tile into shared memory (128-byte swizzle).
+    auto load_q = [&](const Item& x) {
+      const int n = x.hi - x.lo;
+      if (!x.two && s == 1 && n < 2) return;
+      const int tok0 = x.i0 + (x.two ? s * p.tok_tile : 0);
+      const int rows = min(p.tok_tile, x.i0 + x.ntok - tok0) * p.G;
+      constexpr int kChunks = D / 8;
+      const uint16_t* src = p.q + static_cast<long long>(x.first + tok0) * p.q_token +
+                            static_cast<long long>(x.h) * p.G * p.q_head;
+      for (int i = row; i < rows * kChunks; i += kTile) {
+        const int r = i / kChunks, c = i % kChunks;
+        const int tk = r / p.G, g = r - tk * p.G;
+        const uint4 v = ld_ro_v4(src + tk * p.q_token + g * p.q_head + c * 8);
+        *reinterpret_cast<uint4*>(qs + (c >> 3) * Sh::kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->qfull[s]);
+    };
+
+    bool more = __all_sync(0xffffffffu, next_item(0));
+    if (more) load_q(item_at(0));
+    int meta_tail = 0, meta_ends = 0, meta_token = 0, meta_ntok = 0, meta_head = 0;
+    for (int k = 0; more; ++k) {
+      const Item& it = item_at(k);
+      const int n = it.hi - it.lo;
+      const int ns = it.two ? n : (n + 1 - s) / 2;
+      const int tok0 = it.i0 + (it.two ? s * p.tok_tile : 0);
+      const int ntok = min(p.tok_tile, it.i0 + it.ntok - tok0);
+      const int rows = ntok * p.G;
+      const bool busy = (warp & 3) * 32 < rows;  // this warp has rows
+      const bool live = row < rows;
+      const int my_token = tok0 + (live ? rt : 0);
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < ns; ++i) {
+        const int j = it.two ? i : 2 * i + s;
+        ok = __all_sync(0xffffffffu, wait_bar(&sh->sfull[s], s_ph, p.err, abort));
+        if (!ok) break;
+        s_ph ^= 1;
+        tc_fence_after();
+        if (busy) {
+          float x[kTile];
+#pragma unroll
+          for (int c = 0; c < kTile; c += 32) tmem_ld_32(ts + c, x + c);
+          tmem_ld_wait();
+          const int key0 = (it.lo + j) * kTile;
+          if (key0 + kTile > it.full) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t vis = live ? visible(p, it, my_token, key0 + 32 * w) : 0u;
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!((vis >> c) & 1)) x[32 * w + c] = -INFINITY;
+            }
+          }
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int c = 4; c < kTile; c += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx[k] = c + 4 + k < kTile ? fmaxf(fmaxf(mx[k], x[c + k]), x[c + 4 + k]) : fmaxf(mx[k], x[c + k]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          if (i == 0) {
+            m = top;
+          } else if (const bool raise = live && top > m + kRaise; __any_sync(0xffffffffu, raise)) {
+            // each row by its own values alone, whatever the rows beside it do
+            const float f = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx(m - top);
+            m = raise ? top : m;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld_16(to + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st_16(to + c, o);
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : -m;
+          const f2 scale2 = f2_make(p.scale_log2, p.scale_log2), base2 = f2_make(base, base);
+          f2 sum[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+#pragma unroll
+          for (int c = 0; c < kTile; c += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float a, b;
+              f2_split(f2_fma(f2_make(x[c + 2 * k], x[c + 2 * k + 1]), scale2, base2), a, b);
+              a = exp2_approx(a);
+              b = exp2_approx(b);
+              sum[k & 1] = f2_add(sum[k & 1], f2_make(a, b));
+              w[k] = pack_pair<BF16>(a, b);
+            }
+            tmem_st_16(ts + c / 2, w);
+          }
+          float a, b;
+          f2_split(f2_add(sum[0], sum[1]), a, b);
+          l += a + b;
+          tmem_st_wait();
+        }
+        if (i == 0 && o1_pending) {  // O_1 of the item before must have been read
+          ok = __all_sync(0xffffffffu, wait_bar(&sh->o1read, b_ph ^ 1, p.err, abort));
+          if (!ok) break;
+          o1_pending = false;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->pfull[s]);
+      }
+      if (!ok) break;
+      more = __all_sync(0xffffffffu, next_item(k + 1));
+      if (more) load_q(item_at(k + 1));
+
+      // ---- the item's end
+      const bool joined = !it.two && n > 1;  // two streams hold the same rows
+      const bool whole = it.lo == 0 && it.hi == it.nt;
+      const int slot = it.lo > 0 ? 0 : 1;
+      if (!whole) {
+        if (it.lo > 0)
+          meta_ends = it.hi == it.nt;
+        else
+          meta_tail = 1, meta_token = it.first + it.i0, meta_ntok = it.ntok, meta_head = it.h;
+      }
+      if (joined && s == 1) {
+        sh->m1[row] = m;
+        sh->l1[row] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ml1);
+        if (lane == 0) done(k);
+        o_ph ^= 1;
+        b_ph ^= 1;
+        o1_pending = true;
+        continue;
+      }
+      if (!it.two && s == 1) {  // a single key tile: stream 0's alone
+        __syncwarp();
+        if (lane == 0) done(k);
+        continue;
+      }
+      ok = __all_sync(0xffffffffu, wait_bar(&sh->ofull[s], o_ph, p.err, abort));
+      if (!ok) break;
+      o_ph ^= 1;
+      float f0 = 1.f, f1 = 0.f;
+      if (joined) {
+        ok = __all_sync(0xffffffffu, wait_bar(&sh->ml1, b_ph, p.err, abort)) &&
+             __all_sync(0xffffffffu, wait_bar(&sh->ofull[1], o1_ph, p.err, abort));
+        if (!ok) break;
+        const float m1 = sh->m1[row], l1 = sh->l1[row];
+        const float top = fmaxf(m, m1);
+        f0 = m == -INFINITY ? 0.f : exp2_approx(m - top);
+        f1 = m1 == -INFINITY ? 0.f : exp2_approx(m1 - top);
+        l = l * f0 + l1 * f1;
+        m = top;
+        o1_ph ^= 1;
+      } else if (it.two) {
+        o1_ph ^= 1;
+      }
+      tc_fence_after();
+      if (busy) {
+        const bool bad = sh->bad[(k + 1) % kBadSlots] == k + 1;
+        const float norm = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        f0 *= norm;
+        f1 *= norm;
+        const size_t out_row = (static_cast<size_t>(it.first + my_token) * p.Hq + it.h * p.G + rg);
+        const int part_row = (it.two ? s * kTile : 0) + row;
+        float* part = p.part + (static_cast<size_t>(blockIdx.x) * 2 + slot) * Sh::kPartFloats;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld_32(to + c, o);
+          if (joined) {
+            float o1[32];
+            tmem_ld_32(to + D + c, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = o[k] * f0 + o1[k] * f1;
+          } else {
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] *= f0;
+          }
+          if (bad && live) {  // values that were kept out of the MMA
+            for (int key = max(it.full, it.lo * kTile); key < min(it.need, it.hi * kTile); ++key) {
+              if (!(visible(p, it, my_token, key) & 1)) continue;
+              const int page = p.table[static_cast<long long>(it.b) * p.table_stride + (key >> p.page_shift)];
+              if (page < 0 || page >= p.num_pages) continue;
+              const uint16_t* v = p.v + page * p.cs.page + (key & ((1 << p.page_shift) - 1)) * p.cs.row +
+                                  it.h * p.cs.head + c;
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float e = BF16 ? __uint_as_float(static_cast<uint32_t>(v[k]) << 16)
+                                     : __half2float(__ushort_as_half(v[k]));
+                if (!isfinite(e)) o[k] += e;
+              }
+            }
+          }
+          if (!live) continue;
+          if (whole) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * D + c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              dst[k] = make_uint4(pack_pair<BF16>(o[8 * k], o[8 * k + 1]), pack_pair<BF16>(o[8 * k + 2], o[8 * k + 3]),
+                                  pack_pair<BF16>(o[8 * k + 4], o[8 * k + 5]),
+                                  pack_pair<BF16>(o[8 * k + 6], o[8 * k + 7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(part + static_cast<size_t>(part_row) * D + c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        }
+        if (live) {
+          if (!whole) {
+            part[kRowsMax * D + part_row] = m;
+            part[kRowsMax * D + kRowsMax + part_row] = l;
+          } else if (p.lse) {
+            p.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          }
+        }
+      }
+      if (joined) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->o1read);
+        b_ph ^= 1;
+      }
+      __syncwarp();
+      if (lane == 0) done(k);
+    }
+    if (tid == 0) {
+      Meta mt;
+      mt.tail = meta_tail, mt.head_ends = meta_ends, mt.token = meta_token, mt.ntok = meta_ntok, mt.head = meta_head;
+      p.meta[blockIdx.x] = mt;
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort) {  // let the TMA copies still in flight land (they take microseconds)
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) {
+    }
+  }
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partials of the items that lie in several CTAs, in CTA order.  Block
+// (c, y): the item that begins in CTA c and goes on, rows y * kJoinRows on.
+constexpr int kJoinRows = 16, kJoinThreads = 128;
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArgs p, int ctas) {
   constexpr int kPer = D / 32;
   pdl_launch_next();
   pdl_wait_previous();
-  const int lane = threadIdx.x & 31;
-  const long long gw = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int t = static_cast<int>(gw / p.Hq), h = static_cast<int>(gw % p.Hq);
-  if (t >= p.T) return;
-  int b = 0;
-  for (int i = 0; i < p.B; ++i)
-    if (p.cu[i] <= t) b = i;
-  const int first = p.cu[b], n = min(p.cu[b + 1], p.T) - first, i = t - first;
-  const bool live = i < n;
-  const int kv = live ? p.kv_lens[b] : 0, ctx = max(0, kv - n);
-  const int kh = h / (p.Hq / p.Hkv);
-  auto ld = [](const uint16_t* x) {
-    return BF16 ? __uint_as_float(static_cast<uint32_t>(*x) << 16) : __half2float(__ushort_as_half(*x));
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Meta mt = p.meta[c];
+  if (!mt.tail) return;
+  const int rows = mt.ntok * p.G, split = p.tok_tile * p.G;  // rows of the first tile
+  if (static_cast<int>(blockIdx.y) * kJoinRows >= rows) return;
+  int last = c + 1;  // the CTA in which the item ends
+  while (last < ctas - 1 && !p.meta[last].head_ends) ++last;
+  auto partial = [&](int cta) {
+    return p.part + (static_cast<size_t>(cta) * 2 + (cta == c ? 1 : 0)) * Shape<D>::kPartFloats;
   };
-  float q[kPer], acc[kPer], mx = -INFINITY, sum = 0.f;
+  for (int r = blockIdx.y * kJoinRows + warp; r < min(rows, static_cast<int>(blockIdx.y + 1) * kJoinRows);
+       r += kJoinThreads / 32) {
+    const int pr = r < split ? r : kTile + r - split;
+    float top = -INFINITY;
+    for (int k = c + lane; k <= last; k += 32) top = fmaxf(top, partial(k)[kRowsMax * D + pr]);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    q[j] = ld(p.q + t * p.q_token + h * p.q_head + lane + 32 * j) * p.scale;
-    acc[j] = 0.f;
-  }
-  for (int key = 0; key < kv; ++key) {
-    const int node = key - ctx;
-    if (node >= 0) {
-      if (!p.mask ? node > i
-                  : node >= p.mask_words * 64 ||
-                        !((p.mask[static_cast<size_t>(t) * p.mask_words + (node >> 6)] >> (node & 63)) & 1))
-        continue;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float acc[kPer], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+#pragma unroll 4
+    for (int k = c; k <= last; ++k) {
+      const float* src = partial(k);
+      const float m = src[kRowsMax * D + pr];
+      const float w = m == -INFINITY ? 0.f : exp2_approx(m - top);
+      sum += w * src[kRowsMax * D + kRowsMax + pr];
+      if constexpr (kPer == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<size_t>(pr) * D + lane * 4);
+        acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src + static_cast<size_t>(pr) * D + lane * 2);
+        acc[0] += w * v.x, acc[1] += w * v.y;
+      }
     }
-    const int blk = key >> p.page_shift;
-    const int page = blk < p.table_width ? p.table[b * p.table_stride + blk] : -1;
-    if (page < 0 || page >= p.num_pages) {
-      if (lane == 0) atomicOr(p.err, kErrBadIndex);
-      continue;
-    }
-    const size_t at = page * p.cs.page + (key & ((1 << p.page_shift) - 1)) * p.cs.row + kh * p.cs.head;
-    float s = 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t row = static_cast<size_t>(mt.token + r / p.G) * p.Hq + mt.head * p.G + r % p.G;
+    uint32_t w[kPer / 2];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) s += q[j] * ld(p.k + at + lane + 32 * j);
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float nm = fmaxf(mx, s), base = nm == -INFINITY ? 0.f : nm;
-    const float corr = expf(mx - base), pw = expf(s - base);
-    sum = sum * corr + pw;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] = acc[j] * corr + pw * ld(p.v + at + lane + 32 * j);
-    mx = nm;
+    for (int j = 0; j < kPer / 2; ++j) w[j] = pack_pair<BF16>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    if constexpr (kPer == 4)
+      *reinterpret_cast<uint2*>(p.out + row * D + lane * 4) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(p.out + row * D + lane * 2) = w[0];
+    if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* o = p.out + (static_cast<size_t>(t) * p.Hq + h) * D;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    o[lane + 32 * j] = static_cast<uint16_t>(pack_pair<BF16>(sum == 0.f ? 0.f : acc[j] * inv, 0.f) & 0xFFFFu);
-  if (p.lse && lane == 0) p.lse[static_cast<size_t>(t) * p.Hq + h] = sum == 0.f ? -INFINITY : mx + logf(sum);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int make_cache_map(const void* base, const CacheStrides& cs, int D, int rows, int Hkv, int pages, CUtensorMap* m) {
+  auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode_fn());
+  if (!enc) return NG_ERR_CUDA;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(Hkv), static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(cs.row) * 2, static_cast<cuuint64_t>(cs.head) * 2,
+                                 static_cast<cuuint64_t>(cs.page) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kTile)), 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? NG_OK
+             : NG_ERR_CUDA;
+}
+
+constexpr size_t kMetaBytes = 16384;
+size_t attn_workspace_bytes(int D, const DeviceInfo& dev) {
+  const size_t part = D == 128 ? Shape<128>::kPartFloats : Shape<64>::kPartFloats;
+  return kMetaBytes + static_cast<size_t>(dev.sm_count) * 2 * part * sizeof(float);
 }
 
 template <bool BF16, int D>
-int launch_tree_attn(const TreeAttnArgs& a, cudaStream_t st) {
-  const long long warps = static_cast<long long>(a.T) * a.Hq;
-  return launch_chained(tree_attn_simple<BF16, D>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, a);
+int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnArgs& a, const DeviceInfo& dev,
+                     cudaStream_t st) {
+  constexpr int smem = Shape<D>::kSmem + 1024 + static_cast<int>(sizeof(Shared));
+  static_assert(smem <= 227 * 1024, "ring and barriers must fit in shared memory");
+  auto kern = tree_attn_kernel<BF16, D>;
+  static std::once_flag once[kMaxDevices];
+  std::call_once(once[dev.device],
+                 [&] { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  if (int e = launch_chained(kern, dim3(dev.sm_count), dim3(kAttnThreads), smem, st, mk, mv, a)) return e;
+  const int rows = static_cast<int>(std::min<long long>(kRowsMax, static_cast<long long>(a.T) * a.G));
+  return launch_chained(tree_attn_join<BF16, D>, dim3(dev.sm_count, (rows + kJoinRows - 1) / kJoinRows),
+                        dim3(kJoinThreads), 0, st, a, dev.sm_count);
 }
 
 }  // namespace
 }  // namespace ngb
 
 extern "C" size_t ng_tree_attn_workspace_bytes(int D) {
-  if (D != 64 && D != 128) return 0;
-  return 256;
+  using namespace ngb;
+  DeviceInfo dev;
+  if ((D != 64 && D != 128) || current_device_info(&dev) != NG_OK) return 0;
+  return attn_workspace_bytes(D, dev);
 }
 
 extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q_stride_head,
@@ -111,7 +1002,7 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
   if (!q || !k_cache || !v_cache || !block_table || !kv_lens || !cu_new || !out || !workspace)
     return NG_ERR_NULL_POINTER;
   if (!act_dtype_ok(dtype)) return NG_ERR_BAD_DTYPE;
-  if (B < 1 || T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > 128 || (D != 64 && D != 128) ||
+  if (B < 1 || T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > kTile || (D != 64 && D != 128) ||
       num_pages < 1 || table_width < 1 || table_stride < table_width || !page_size_ok(page_size) ||
       static_cast<long long>(T) * Hq > (1LL << 30))
     return NG_ERR_BAD_SHAPE;
@@ -120,20 +1011,27 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
     return NG_ERR_BAD_SHAPE;
   if (!(scale > 0.f) || !(scale < INFINITY) || mask_words < 0 || (mask && mask_words < 1))
     return NG_ERR_BAD_ARGUMENT;
-  if (workspace_bytes < ng_tree_attn_workspace_bytes(D)) return NG_ERR_BAD_ARGUMENT;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) ||
       !aligned(mask, 8) || !aligned(workspace, 256))
     return NG_ERR_MISALIGNED;
   DeviceInfo dev;
   if (int st = current_device_info(&dev)) return st;
+  if (workspace_bytes < attn_workspace_bytes(D, dev)) return NG_ERR_BAD_ARGUMENT;
+  CUtensorMap mk, mv;
+  if (int st = make_cache_map(k_cache, cs, D, page_size, Hkv, num_pages, &mk)) return st;
+  if (int st = make_cache_map(v_cache, cs, D, page_size, Hkv, num_pages, &mv)) return st;
+  const int G = Hq / Hkv;
   const TreeAttnArgs a{static_cast<const uint16_t*>(q), q_stride_token, q_stride_head,
-                       static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache), cs,
-                       block_table, table_stride, table_width, kv_lens, cu_new,
-                       reinterpret_cast<const unsigned long long*>(mask), mask_words,
-                       static_cast<uint16_t*>(out), lse, B, T, Hq, Hkv, num_pages, log2_of(page_size), scale,
-                       dev.err};
+                       static_cast<const uint16_t*>(v_cache), cs, block_table, table_stride, table_width, kv_lens,
+                       cu_new, reinterpret_cast<const unsigned long long*>(mask), mask_words,
+                       static_cast<uint16_t*>(out), lse, B, T, Hq, Hkv, G, kTile / G, num_pages,
+                       log2_of(page_size), 4, scale * 1.4426950408889634f,
+                       reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kMetaBytes),
+                       static_cast<Meta*>(workspace), dev.err};
   auto st = static_cast<cudaStream_t>(stream);
   if (D == 128)
-    return dtype == NG_DTYPE_BF16 ? launch_tree_attn<true, 128>(a, st) : launch_tree_attn<false, 128>(a, st);
-  return dtype == NG_DTYPE_BF16 ? launch_tree_attn<true, 64>(a, st) : launch_tree_attn<false, 64>(a, st);
+    return dtype == NG_DTYPE_BF16 ? launch_tree_attn<true, 128>(mk, mv, a, dev, st)
+                                  : launch_tree_attn<false, 128>(mk, mv, a, dev, st);
+  return dtype == NG_DTYPE_BF16 ? launch_tree_attn<true, 64>(mk, mv, a, dev, st)
+                                : launch_tree_attn<false, 64>(mk, mv, a, dev, st);
 }
