@@ -135,14 +135,48 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc].
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// One lane of a converged warp.  The MMA warp runs converged, with operands that
+// are the same in all lanes, and issues under this predicate: the compiler then
+// keeps them in uniform registers, which tcgen05 instructions take.  (Issued from
+// a "lane 0" branch instead, every MMA took 140 cycles, twice the tensor core's time.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Shared-memory matrix descriptors, low words (start address >> 4, leading offset
+// >> 4 from bit 16) and the high word that both kinds share: stride offset 1024 B
+// (eight 128-byte rows), version 1, 128-byte swizzle.
+//   K-major (Q, K): rows of 64 values; the leading offset is not used.
+//   N-major (V as the B operand, N = the D values contiguous): 8 keys per atom, the
+//   stride offset steps along the keys, the leading offset to the next 64 values.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr, uint32_t half_bytes) {
+  return (addr >> 4) | ((half_bytes >> 4) << 16);
+}
+
+// D[tmem] (+)= A * B, descriptors by their low words; A from shared / from tensor memory.
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .b64 x, y;\n\t.reg .pred p;\n\t"
+      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "n"(kAccumulate ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .b64 y;\n\t.reg .pred p;\n\t"
+      "mov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -177,19 +211,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   f2 d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-
-// V tile as the MMA's B operand, N (the D values) contiguous: rows of 64 values
-// (128 bytes, 128-byte swizzle), 8 keys per 1024-byte atom.  Stride offset: atoms
-// along the keys, 1024 B; leading offset: the next 64 values, one half on.
-__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t addr, uint32_t half_bytes) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(half_bytes >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
   return d;
 }
 
@@ -467,58 +488,76 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    {
       constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kTile);
       constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
       uint32_t base = 0;       // ring places used by earlier items
       uint32_t clean_ph = 0;   // per stage: parity of its next cleaned use
       uint32_t q_ph = 0, p_ph = 0;  // parities, bit s
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
+      auto wait_all = [&](uint64_t* bar, uint32_t ph, unsigned int* err, volatile int* ab) -> bool {
+        return __all_sync(0xffffffffu, wait_bar(bar, ph, err, ab));
+      };
       bool ok = true;
-      for (int k = 0; ok && next_item(k); ++k) {
+      for (int k = 0; ok && __all_sync(0xffffffffu, next_item(k)); ++k) {
         const Item& it = item_at(k);
-        const int n = it.hi - it.lo, lo = it.lo, full = it.full;
-        const bool two = it.two;
-        done(k);
+        // broadcasts: known to be the same in all lanes
+        const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
+        const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
+        const bool two = __shfl_sync(0xffffffffu, it.two, 0);
+        if (lane == 0) done(k);
         const int n0 = two ? n : (n + 1) / 2, n1 = two ? n : n / 2;
         auto scores = [&](int s, int i) {  // S_s = Q_s K^T of the stream's i-th tile
           const int j = two ? i : 2 * i + s;
           const uint32_t pl = base + k_place(two, j);
           const uint32_t st = pl % kStages;
-          if (!wait_bar(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          if (!wait_all(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
           tc_fence_after();
-          const uint32_t qa = smem_u32(smem + s * Sh::kTileBytes), ka = smem_u32(ring + st * Sh::kTileBytes);
+          const uint32_t qd = q_desc + s * (Sh::kTileBytes >> 4);
+          const uint32_t kd = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring) + st * Sh::kTileBytes), 0);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * Sh::kHalfBytes + (kk & 3) * 32;
-            umma_f16(tmem + s * kTile, sw128_kmajor_desc(qa + o), sw128_kmajor_desc(ka + o), idesc_s, kk != 0);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * Sh::kHalfBytes + (kk & 3) * 32) >> 4;
+              if (kk == 0)
+                mma_ss<false>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
+              else
+                mma_ss<true>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
+            }
+            umma_commit(&sh->sfull[s]);
+            if (!two || s == 1) umma_commit(&sh->empty[st]);
           }
-          umma_commit(&sh->sfull[s]);
-          if (!two || s == 1) umma_commit(&sh->empty[st]);
+          __syncwarp();
           return true;
         };
         auto values = [&](int s, int i) {  // O_s += P_s V
           const int j = two ? i : 2 * i + s;
           const uint32_t pl = base + v_place(two, j, n);
           const uint32_t st = pl % kStages;
-          if (!wait_bar(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          if (!wait_all(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
           if ((lo + j + 1) * kTile > full) {
-            if (!wait_bar(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort)) return false;
+            if (!wait_all(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort)) return false;
             if (!two || s == 1) clean_ph ^= 1u << st;
           }
           tc_fence_after();
-          const uint32_t va = smem_u32(ring + st * Sh::kTileBytes);
+          const uint32_t vd =
+              __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring) + st * Sh::kTileBytes, Sh::kHalfBytes), 0);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            umma_f16_ts(tmem + 2 * kTile + s * D, tmem + s * kTile + kk * 8,
-                        sw128_nmajor_desc(va + kk * 2048, Sh::kHalfBytes), idesc_o, (i | kk) != 0);
-          if (!two || s == 1) umma_commit(&sh->empty[st]);
-          if (i == (s ? n1 : n0) - 1) umma_commit(&sh->ofull[s]);
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              mma_ts(tmem_u + 2 * kTile + s * D, tmem_u + s * kTile + kk * 8, vd + kk * (2048 >> 4), idesc_o,
+                     (i | kk) != 0);
+            if (!two || s == 1) umma_commit(&sh->empty[st]);
+            if (i == (s ? n1 : n0) - 1) umma_commit(&sh->ofull[s]);
+          }
+          __syncwarp();
           return true;
         };
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (ok && (s ? n1 : n0) > 0) {
-            ok = wait_bar(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
+            ok = wait_all(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
             q_ph ^= 1u << s;
             ok = ok && scores(s, 0);
           }
@@ -527,7 +566,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int s = 0; s < 2; ++s) {
             const int mine_n = s ? n1 : n0;
             if (ok && i < mine_n) {
-              ok = wait_bar(&sh->pfull[s], (p_ph >> s) & 1, p.err, abort);
+              ok = wait_all(&sh->pfull[s], (p_ph >> s) & 1, p.err, abort);
               p_ph ^= 1u << s;
               ok = ok && values(s, i);
               if (ok && i + 1 < mine_n) ok = scores(s, i + 1);
