@@ -7,25 +7,22 @@
 // The query heads that share a KV head are rows of one tile: row r of a tile is
 // token r / G, head r % G (G = Hq / Hkv), so K and V are read once for all of them
 // and a tile of 128 rows holds 128 / G tokens.  A work item is (request, KV head,
-// two tiles of tokens); its keys come in tiles of 64.
+// two tiles of tokens); its keys come in tiles of 128.
 //
 // One persistent CTA per SM, warp-specialised:
-//   warps 0-3, 4-7  softmax of stream 0 and stream 1, one thread per row
-//   warp 8          TMA: the pages of a K and a V tile into a ring of stages, one lane per
+//   warps 0-7, 8-15 softmax of stream 0 and stream 1: two threads per row, 64 keys each
+//   warp 16         TMA: the pages of a K or V tile into a ring of stages, one lane per
 //                   page and 64-value half, 128-byte swizzle
-//   warps 9, 11     tcgen05.mma: S_s = Q_s K^T (128 x 64, both operands from shared
+//   warp 17         tcgen05.mma: S_s = Q_s K^T (128 x 128, both operands from shared
 //                   memory), O_s += P_s V (P_s from tensor memory)
-//   warp 10         tensor-memory allocation; walks this CTA's share of the work and hands
-//                   out its items; rows of V that no MMA may see (below)
-// Tensor memory: two buffers of scores for each stream (64 columns each; P is written over
-// the scores it comes from), O_0, O_1 (D each).  While the softmax has one tile of scores the
-// tensor core computes the next one into the other buffer, so neither waits for
-// the other.  (With one buffer of 128 keys the scores of the next tile had to wait for P V of
-// this one: a chain of softmax and both products, 4400 cycles for two tiles of 128
-// queries x 128 keys, of which the tensor core worked 2100.)
-// With two tiles of tokens both streams go through every key tile (which is loaded
-// once); with one tile they take the even and the odd key tiles, each with a softmax
-// state of its own, and stream 0 joins the two at the end.
+//   warp 18         tensor-memory allocation; rows of V that no MMA may see (below)
+//   warp 19         walks this CTA's share of the work and hands out its items
+// The two streams hide each other's softmax: while one is in its exponentials the
+// tensor core works for the other.  With two tiles of tokens both streams go
+// through every key tile (which is loaded once); with one tile they take the even
+// and the odd key tiles, each with a softmax state of its own, and stream 0 joins
+// the two at the end.  Tensor memory: S_0, S_1 (128 columns each; P_s is written over S_s), O_0,
+// O_1 (D each).
 //
 // Work is split evenly over the CTAs: every CTA adds up the key tiles of all items
 // (from the lengths, on the GPU; an item counts one more for its fixed cost) and
@@ -54,15 +51,15 @@
 namespace ngb {
 namespace {
 
-constexpr int kTile = 128;         // rows of a query tile
-constexpr int kKeys = 64;          // keys of a key tile
+constexpr int kTile = 128;         // rows of a query tile, keys of a key tile
 constexpr int kAttnThreads = 384;  // 12 warps
+constexpr int kChunk = 64;         // scores that a softmax thread holds at a time
 constexpr int kRowsMax = 2 * kTile;
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
 constexpr int kBadSlots = 8;
 constexpr int kItems = 4;          // work items handed out ahead
-constexpr int kMinUnits = 8;       // least work of a CTA, in key tiles
-constexpr int kItemUnits = 2;      // what an item costs beside its key tiles, in key tiles
+constexpr int kMinUnits = 4;       // least work of a CTA, in key tiles
+constexpr int kItemUnits = 1;      // what an item costs beside its key tiles, in key tiles
 
 // A work item as one CTA sees it.
 struct alignas(16) Item {
@@ -77,30 +74,12 @@ struct alignas(16) Item {
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kQBytes = kTile * D * 2, kQHalf = kTile * 128;   // a Q tile, its 64-value half
-  static constexpr int kKvBytes = kKeys * D * 2, kKvHalf = kKeys * 128; // a K or V tile
-  static constexpr int kStageBytes = 2 * kKvBytes;                      // K, then V
-  static constexpr int kStages = D == 128 ? 5 : 10;                     // ring: 160 KB
-  static constexpr int kSmem = 2 * kQBytes + kStages * kStageBytes;
+  static constexpr int kTileBytes = kTile * D * 2;           // a Q, K or V tile
+  static constexpr int kHalfBytes = kTile * 128;             // its 64-value half
+  static constexpr int kStages = D == 128 ? 5 : 10;          // ring: 160 KB
+  static constexpr int kSmem = (2 + kStages) * kTileBytes;
   // One partial: kRowsMax rows of D values, maxima, sums.
   static constexpr size_t kPartFloats = static_cast<size_t>(kRowsMax) * (D + 2);
-};
-
-template <int kStages>
-struct alignas(16) Shared {
-  uint64_t full[kStages], empty[kStages], vissued[kStages], vclean[kStages];
-  uint64_t qfull[2], ofull[2], olast[2];  // olast: all but the last P V of a stream are done
-  uint64_t sfull[2][2], pfull[2][2];       // [stream][buffer]
-  uint64_t ml1, o1read, mma_go, mma_back;
-  uint64_t item_full[kItems], item_empty[kItems];
-  Item items[kItems];
-  long long warp_sum[kAttnThreads / 32];
-  long long start_u;
-  int start_b, start_off;
-  uint32_t tmem;
-  int abort;
-  int bad[kBadSlots];
-  float m1[kTile], l1[kTile];        // stream 1's maxima and sums, for stream 0
 };
 
 // What the joining kernel needs to know of a CTA.
@@ -125,11 +104,117 @@ struct TreeAttnArgs {
   int mask_words;
   uint16_t* out;
   float* lse;
-  int B, T, Hq, Hkv, G, tok_tile, num_pages, page_shift, min_units;
+  int B, T, Hq, Hkv, G, tok_tile, num_pages, page_shift;
   float scale_log2;
   float* part;
   Meta* meta;
   unsigned int* err;
+};
+
+// ---------------------------------------------------------------------------
+// The line of work
+// ---------------------------------------------------------------------------
+struct Request {
+  int first, n, kv, ctx;
+};
+
+__device__ __forceinline__ Request load_request(const TreeAttnArgs& p, int b) {
+  Request r;
+  r.first = min(max(p.cu[b], 0), p.T);
+  r.n = min(max(p.cu[b + 1], r.first), p.T) - r.first;
+  const long long most = static_cast<long long>(p.table_width) << p.page_shift;
+  r.kv = max(p.kv_lens[b], 0);
+  if (r.kv > most) {  // more rows than its table names
+    atomicOr(p.err, kErrBadIndex);
+    r.kv = static_cast<int>(most);
+  }
+  r.ctx = max(0, r.kv - r.n);
+  return r;
+}
+
+// Keys that the tokens [i0, i1) need, and the leading ones that all of them see.
+__device__ __forceinline__ int keys_needed(const TreeAttnArgs& p, const Request& r, int i1) {
+  return p.mask ? r.kv : min(r.kv, r.ctx + i1);
+}
+__device__ __forceinline__ int keys_full(const TreeAttnArgs& p, const Request& r, int i0) {
+  return p.mask ? r.ctx : min(r.kv, r.ctx + i0 + 1);
+}
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
+
+// Units of one KV head of a request: its tiles, and kItemUnits for each item.
+__device__ __forceinline__ long long head_units(const TreeAttnArgs& p, const Request& r) {
+  const int step = 2 * p.tok_tile;
+  if (p.mask) return static_cast<long long>((r.n + step - 1) / step) * (tiles_of(r.kv) + kItemUnits);
+  long long u = 0;
+  for (int i0 = 0; i0 < r.n; i0 += step) u += tiles_of(keys_needed(p, r, min(r.n, i0 + step))) + kItemUnits;
+  return u;
+}
+
+// a / b for 0 <= a, 0 < b; the 64-bit division is several times as long as the other.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if ((a | b) >> 32) return a / b;
+  return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+}
+
+// A CTA's way along the line.
+struct Walk {
+  long long u, u1;  // next unit, end of the share
+  int b, h, i0;     // item that u lies in: request, KV head, first token
+  int off;          // units of it before u
+  int loaded;       // whether r is request b's
+  Request r;
+
+  __device__ __forceinline__ bool next(const TreeAttnArgs& p, Item& it) {
+    const int step = 2 * p.tok_tile;
+    while (u < u1 && b < p.B) {
+      if (!loaded) r = load_request(p, b);
+      loaded = 1;
+      if (r.n == 0) {
+        ++b;
+        loaded = 0;
+        continue;
+      }
+      const int i1 = min(r.n, i0 + step);
+      const int need = keys_needed(p, r, i1);
+      const int nt = tiles_of(need);
+      const int take = static_cast<int>(min(static_cast<long long>(nt + kItemUnits - off), u1 - u));
+      it.b = b, it.h = h, it.i0 = i0, it.ntok = i1 - i0;
+      it.first = r.first, it.ctx = r.ctx, it.kv = r.kv, it.need = need, it.full = keys_full(p, r, i0);
+      it.nt = nt, it.lo = max(0, off - kItemUnits), it.hi = off + take - kItemUnits;
+      it.two = it.ntok > p.tok_tile;
+      u += take;
+      off += take;
+      if (off == nt + kItemUnits) {
+        off = 0;
+        i0 += step;
+        if (i0 >= r.n) {
+          i0 = 0;
+          if (++h == p.Hkv) {
+            h = 0;
+            ++b;
+            loaded = 0;  // when the next item is asked for: this one should not wait for it
+          }
+        }
+      }
+      if (it.hi > it.lo) return true;
+    }
+    return false;
+  }
+};
+
+template <int kStages>
+struct alignas(16) Shared {
+  uint64_t full[kStages], empty[kStages], vissued[kStages], vclean[kStages];
+  uint64_t qfull[2], sfull[2], pfull[2], ofull[2];
+  uint64_t ml1, o1read;
+  uint64_t item_full[kItems], item_empty[kItems];
+  Item items[kItems];
+  long long warp_sum[kAttnThreads / 32];
+  Walk start;                        // where this CTA's share begins
+  uint32_t tmem;
+  int abort;
+  int bad[kBadSlots];
+  float m1[kTile], l1[kTile];        // stream 1's maxima and sums, for stream 0
 };
 
 // ---------------------------------------------------------------------------
@@ -170,19 +255,14 @@ __device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr, uint32_t half_byt
   return (addr >> 4) | ((half_bytes >> 4) << 16);
 }
 
-// Keeps the compiler from computing the operands of all products of an item ahead
-// of its loop, which takes more registers than the warp has.
-__device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b, uint32_t& c) {
-  asm volatile("" : "+r"(a), "+r"(b), "+r"(c));
-}
-
 // D[tmem] (+)= A * B, descriptors by their low words; A from shared / from tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .b64 x, y;\n\t.reg .pred p;\n\t"
       "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(accumulate)
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "n"(kAccumulate ? 1 : 0)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -228,19 +308,6 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   return d;
 }
 
-// Whether a phase has completed, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // Bounded wait of one lane; false once the CTA has given up.  The hint lets the
 // hardware hold the lane for up to 10 ms instead of having it poll: the polls of 16
 // waiting warps made every barrier operation of the MMA warp take three times as long.
@@ -273,89 +340,12 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, unsign
   return __all_sync(0xffffffffu, wait_bar(bar, parity, err, abort));
 }
 
-// ---------------------------------------------------------------------------
-// The line of work
-// ---------------------------------------------------------------------------
-struct Request {
-  int first, n, kv, ctx;
-};
-
-__device__ __forceinline__ Request load_request(const TreeAttnArgs& p, int b) {
-  Request r;
-  r.first = min(max(p.cu[b], 0), p.T);
-  r.n = min(max(p.cu[b + 1], r.first), p.T) - r.first;
-  const long long most = static_cast<long long>(p.table_width) << p.page_shift;
-  r.kv = max(p.kv_lens[b], 0);
-  if (r.kv > most) {  // more rows than its table names
-    atomicOr(p.err, kErrBadIndex);
-    r.kv = static_cast<int>(most);
-  }
-  r.ctx = max(0, r.kv - r.n);
-  return r;
+// Place of key tile j (of n) in the order in which the tiles are loaded: with two
+// query tiles K0 V0 K1 V1 ..., with one K0 K1 V0 K2 V1 ... (the order of the MMAs).
+__device__ __forceinline__ int k_place(bool two, int j) { return two ? 2 * j : (j ? 2 * j - 1 : 0); }
+__device__ __forceinline__ int v_place(bool two, int j, int n) {
+  return two ? 2 * j + 1 : (j == n - 1 ? 2 * n - 1 : 2 * j + 2);
 }
-
-// Keys that the tokens [i0, i1) need, and the leading ones that all of them see.
-__device__ __forceinline__ int keys_needed(const TreeAttnArgs& p, const Request& r, int i1) {
-  return p.mask ? r.kv : min(r.kv, r.ctx + i1);
-}
-__device__ __forceinline__ int keys_full(const TreeAttnArgs& p, const Request& r, int i0) {
-  return p.mask ? r.ctx : min(r.kv, r.ctx + i0 + 1);
-}
-__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kKeys - 1) / kKeys); }
-
-// Units of one KV head of a request: its tiles, and kItemUnits for each item.
-__device__ __forceinline__ long long head_units(const TreeAttnArgs& p, const Request& r) {
-  const int step = 2 * p.tok_tile;
-  if (p.mask) return static_cast<long long>((r.n + step - 1) / step) * (tiles_of(r.kv) + kItemUnits);
-  long long u = 0;
-  for (int i0 = 0; i0 < r.n; i0 += step) u += tiles_of(keys_needed(p, r, min(r.n, i0 + step))) + kItemUnits;
-  return u;
-}
-
-struct Walk {
-  long long u, u1;
-  int b, h, i0;
-  int off;
-  Request r;
-
-  __device__ __forceinline__ bool next(const TreeAttnArgs& p, Item& it) {
-    const int step = 2 * p.tok_tile;
-    while (u < u1 && b < p.B) {
-      if (r.n == 0) {
-        if (++b < p.B) r = load_request(p, b);
-        continue;
-      }
-      const int i1 = min(r.n, i0 + step);
-      const int need = keys_needed(p, r, i1);
-      const int nt = tiles_of(need);
-      const int take = static_cast<int>(min(static_cast<long long>(nt + kItemUnits - off), u1 - u));
-      it.b = b, it.h = h, it.i0 = i0, it.ntok = i1 - i0;
-      it.first = r.first, it.ctx = r.ctx, it.kv = r.kv, it.need = need, it.full = keys_full(p, r, i0);
-      it.nt = nt, it.lo = max(0, off - kItemUnits), it.hi = off + take - kItemUnits;
-      it.two = it.ntok > p.tok_tile;
-      u += take;
-      off += take;
-      if (off == nt + kItemUnits) {
-        off = 0;
-        i0 += step;
-        if (i0 >= r.n) {
-          i0 = 0;
-          if (++h == p.Hkv) {
-            h = 0;
-            if (++b < p.B) r = load_request(p, b);
-          }
-        }
-      }
-      if (it.hi > it.lo) return true;
-    }
-    return false;
-  }
-};
-
-// A stage of the ring holds V of tile j and K of tile j + lead: what the MMA warp
-// takes together, P V of tile j and then the scores two tiles on in the same
-// stream, which take the place of the P just used.  The first `lead` stages of an item hold K alone.
-__device__ __forceinline__ int lead_of(bool two, int n) { return min(two ? 2 : 4, n); }
 
 // 32 bits of token row `row`'s mask from bit `at` on (which may be negative).
 __device__ __forceinline__ uint32_t mask_window(const TreeAttnArgs& p, int row, int at) {
@@ -386,7 +376,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   using Sh = Shape<D>;
   constexpr int kStages = Sh::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];  // 1024: the swizzle atom
-  unsigned char* ring = smem + 2 * Sh::kQBytes;  // after Q_0, Q_1
+  unsigned char* ring = smem + 2 * Sh::kTileBytes;  // after Q_0, Q_1
   auto* sh = reinterpret_cast<Shared<kStages>*>(smem + Sh::kSmem);
   volatile int* abort = &sh->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -394,29 +384,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->empty[s], 2);  // both MMA warps, or one and the TMA warp
+      mbar_init(&sh->empty[s], 1);
       mbar_init(&sh->vissued[s], 1);
       mbar_init(&sh->vclean[s], 1);
     }
     for (int s = 0; s < kItems; ++s) {
       mbar_init(&sh->item_full[s], 1);
-      mbar_init(&sh->item_empty[s], 12);  // every warp
+      mbar_init(&sh->item_empty[s], 11);  // TMA, MMA, V rows, 8 softmax warps
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh->qfull[s], 4);
+      mbar_init(&sh->sfull[s], 1);
+      mbar_init(&sh->pfull[s], 4);
       mbar_init(&sh->ofull[s], 1);
-      mbar_init(&sh->olast[s], 1);
-      for (int b = 0; b < 2; ++b) {
-        mbar_init(&sh->sfull[s][b], 1);
-        mbar_init(&sh->pfull[s][b], 4);
-      }
     }
     mbar_init(&sh->ml1, 4);
-    mbar_init(&sh->mma_go, 1);
-    mbar_init(&sh->mma_back, 1);
     mbar_init(&sh->o1read, 4);
     sh->abort = 0;
-    sh->start_b = p.B;
+    sh->start.u = sh->start.u1 = 0;  // no work, unless a thread finds some below
     for (int i = 0; i < kBadSlots; ++i) sh->bad[i] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_k);
@@ -429,8 +414,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   // ---- this CTA's share of the line
   const int per = (p.B + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  const int tokens = min(max(p.cu[p.B], 0), p.T);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += head_units(p, load_request(p, b)) * p.Hkv;
+  Request req = {0, 0, 0, 0};
+  for (int b = b0; b < b1; ++b) {
+    req = load_request(p, b);
+    mine += head_units(p, req) * p.Hkv;
+  }
   long long inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -447,30 +437,44 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if (w < warp) before += sh->warp_sum[w];
     total += sh->warp_sum[w];
   }
-  // Shares of at least min_units: the last CTAs stay idle when there is little work.
-  const long long ctas = min(static_cast<long long>(gridDim.x), max(1ll, total / p.min_units));
-  const long long u0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
-  const long long u1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+  // Shares of at least kMinUnits: the last CTAs stay idle when there is little work.
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1ll, total / kMinUnits)));
+  const long long each = quotient(total, ctas), rest = total - each * ctas;
+  const int c = min(static_cast<int>(blockIdx.x), ctas);
+  const long long u0 = each * c + min(static_cast<long long>(c), rest);
+  const long long u1 = c < ctas ? u0 + each + (c < rest) : u0;
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      const long long units = head_units(p, load_request(p, b)) * p.Hkv;
-      if (u0 < at + units) {
-        sh->start_b = b;
-        sh->start_u = u0 - at;
-        break;
-      }
-      at += units;
+    Walk w;
+    w.u = u0, w.u1 = u1, w.loaded = 1;
+    long long o = u0 - before, hu = 0;
+    for (w.b = b0;; ++w.b) {
+      if (b1 - b0 > 1) req = load_request(p, w.b);
+      hu = head_units(p, req);
+      if (o < hu * p.Hkv) break;
+      o -= hu * p.Hkv;
     }
+    w.r = req;
+    w.h = static_cast<int>(quotient(o, hu));
+    o -= w.h * hu;
+    const int step = 2 * p.tok_tile;
+    w.i0 = 0;
+    for (;;) {
+      const int units = tiles_of(keys_needed(p, req, min(req.n, w.i0 + step))) + kItemUnits;
+      if (o < units) break;
+      o -= units;
+      w.i0 += step;
+    }
+    w.off = static_cast<int>(o);
+    sh->start = w;
   }
+  __syncthreads();
   // rows beyond the last request's tokens see nothing
-  for (long long i = static_cast<long long>(blockIdx.x) * kAttnThreads + tid +
-                     static_cast<long long>(min(max(p.cu[p.B], 0), p.T)) * p.Hq * (D / 8);
+  for (long long i = static_cast<long long>(tokens) * p.Hq * (D / 8) +
+                     static_cast<long long>(blockIdx.x) * kAttnThreads + tid;
        i < static_cast<long long>(p.T) * p.Hq * (D / 8); i += static_cast<long long>(gridDim.x) * kAttnThreads) {
     reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
     if (p.lse && i % (D / 8) == 0) p.lse[i / (D / 8)] = -INFINITY;
   }
-  __syncthreads();
   const uint32_t tmem = sh->tmem;
 
   // The item that is k-th in this CTA: waits for it; false when there is none (or
@@ -483,41 +487,38 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
-    const int shift = min(p.page_shift, 6);  // rows of a piece: a page, or a whole tile of one
-    const int pieces = kKeys >> shift;
-    const bool is_v = lane >= 16;
-    const int piece = (lane & 15) % pieces, half = (lane & 15) / pieces;
+    const int shift = min(p.page_shift, 7);         // rows of a piece: a page, or a whole tile of one
+    const int pieces = kTile >> shift;
+    const int piece = lane % pieces, half = lane / pieces;
     const uint32_t piece_bytes = 128u << shift;
-    const uint32_t offset = (is_v ? Sh::kKvBytes : 0) + half * Sh::kKvHalf + piece * piece_bytes;
+    const uint32_t offset = half * Sh::kHalfBytes + piece * piece_bytes;
     const int page_mask = (1 << p.page_shift) - 1;
-    uint32_t st = 0, ph = 0;  // stage and parity of the next place
+    uint32_t it_count = 0;
     bool ok = true;
     for (int k = 0; ok && next_item(k); ++k) {
       const Item it = item_at(k);
       __syncwarp();
       if (lane == 0) done(k);
-      const int n = it.hi - it.lo, lead = lead_of(it.two, n);
+      const int n = it.hi - it.lo;
       const int* row = p.table + static_cast<long long>(it.b) * p.table_stride;
-      // This lane's key tile at place `pl` of the item, and the page of its piece.
-      auto key_at = [&](int pl) { return (it.lo + (is_v ? pl - lead : pl)) * kKeys + (piece << shift); };
-      auto active_at = [&](int pl) {
-        const int j = is_v ? pl - lead : pl;
-        return half < Sh::kHalves && j >= 0 && j < n && key_at(pl) < it.need;
+      auto active_at = [&](int j) {
+        return half < Sh::kHalves && (it.lo + j) * kTile + (piece << shift) < it.need;
       };
-      auto page_at = [&](int pl) { return active_at(pl) ? row[key_at(pl) >> p.page_shift] : 0; };
-      int page = page_at(0);
-      for (int pl = 0; pl < n + lead; ++pl) {
-        const int page_next = page_at(pl + 1);
-        ok = wait_warp(&sh->empty[st], ph ^ 1, p.err, abort);
-        if (!ok) break;
-        const bool active = active_at(pl);
+      auto page_at = [&](int j) -> int {
+        if (j >= n || !active_at(j)) return 0;
+        return row[((it.lo + j) * kTile + (piece << shift)) >> p.page_shift];
+      };
+      auto load = [&](bool is_v, int j, int page) {
+        const uint32_t s = it_count % kStages, ph = (it_count / kStages) & 1;
+        ++it_count;
+        if (!wait_warp(&sh->empty[s], ph ^ 1, p.err, abort)) return false;
+        const bool active = active_at(j);
         const unsigned votes = __ballot_sync(0xffffffffu, active);
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->full[st], __popc(votes) * piece_bytes);
-          // From here on the parity of full[st] means this use to the V-row warp, which
+          mbar_arrive_expect_tx(&sh->full[s], __popc(votes) * piece_bytes);
+          // From here on the parity of full[s] means this use to the V-row warp, which
           // only looks at some uses and could take another for it.
-          if (pl >= lead && (it.lo + pl - lead + 1) * kKeys > it.full) mbar_arrive(&sh->vissued[st]);
-          if (!it.two) mbar_arrive(&sh->empty[st]);  // only one MMA warp will release it
+          if (is_v && (it.lo + j + 1) * kTile > it.full) mbar_arrive(&sh->vissued[s]);
         }
         __syncwarp();
         if (active) {
@@ -525,190 +526,144 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             atomicOr(p.err, kErrBadIndex);
             page = p.num_pages;
           }
-          tma_load_4d(smem_u32(ring + st * Sh::kStageBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[st],
-                      half * 64, key_at(pl) & page_mask, it.h, page);
+          const int r = ((it.lo + j) * kTile + (piece << shift)) & page_mask;
+          tma_load_4d(smem_u32(ring + s * Sh::kTileBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[s],
+                      half * 64, r, it.h, page);
         }
-        page = page_next;
-        if (++st == kStages) st = 0, ph ^= 1;
+        return true;
+      };
+      const int lag = it.two ? 0 : 1;
+      int pg = page_at(0), pg_prev = 0;
+      for (int j = 0; ok && j < n + lag; ++j) {
+        const int pg_next = page_at(j + 1);
+        if (j < n) ok = load(false, j, pg);
+        if (ok && j >= lag) ok = load(true, j - lag, lag ? pg_prev : pg);
+        pg_prev = pg;
+        pg = pg_next;
       }
     }
-  } else if (warp == 9 || warp == 11) {
-    // ------------------------------------------------------------ MMA issuers
-    // With two tiles of tokens warp 9 issues stream 0 and warp 11 stream 1: the barrier
-    // operations between two groups of products cost the issuing warp as much time as
-    // the products take.  Items of one tile of tokens are warp 9's alone.
-    constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kKeys);
-    constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
-    const int role = warp == 11;
-    uint32_t st = 0, ph = 0;        // stage and parity of the next place
-    uint32_t clean_ph = 0;          // per stage: parity of its next cleaned use
-    uint32_t q_ph = 0, p_ph = 0;    // parities of Q (bit s) and P (bit 2 s + buffer)
-    uint32_t pair_ph = 0;           // parity of mma_go (warp 11) or mma_back (warp 9)
-    bool was_two = false;
-    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-    const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
-    const uint32_t ring_k = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring)), 0);
-    const uint32_t ring_v =
-        __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring) + Sh::kKvBytes, Sh::kKvHalf), 0);
-    // One elected lane: S_s = Q_s K^T into buffer b with K in the current stage.
-    auto issue_scores = [&](int s, int b) {
-      uint32_t d = tmem_u + s * (2 * kKeys) + b * kKeys;
-      uint32_t qd = q_desc + s * (Sh::kQBytes >> 4), kd = ring_k + st * (Sh::kStageBytes >> 4);
-      opaque(d, qd, kd);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    {
+      constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kTile);
+      constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
+      uint32_t base = 0;       // ring places used by earlier items
+      uint32_t clean_ph = 0;   // per stage: parity of its next cleaned use
+      uint32_t q_ph = 0, p_ph = 0;  // parities, bit s
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
+      bool ok = true;
+      for (int k = 0; ok && next_item(k); ++k) {
+        const Item& it = item_at(k);
+        // broadcasts: known to be the same in all lanes
+        const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
+        const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
+        const bool two = __shfl_sync(0xffffffffu, it.two, 0);
+        if (lane == 0) done(k);
+        const int n0 = two ? n : (n + 1) / 2, n1 = two ? n : n / 2;
+        auto scores = [&](int s, int i) {  // S_s = Q_s K^T of the stream's i-th tile
+          const int j = two ? i : 2 * i + s;
+          const uint32_t pl = base + k_place(two, j);
+          const uint32_t st = pl % kStages;
+          if (!wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          tc_fence_after();
+          const uint32_t qd = q_desc + s * (Sh::kTileBytes >> 4);
+          const uint32_t kd = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring) + st * Sh::kTileBytes), 0);
+          if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        mma_ss(d, qd + (((kk >> 2) * Sh::kQHalf + (kk & 3) * 32) >> 4),
-               kd + (((kk >> 2) * Sh::kKvHalf + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
-      umma_commit(&sh->sfull[s][b]);
-    };
-    auto advance = [&](int places) {
-      st += places;
-      while (st >= kStages) st -= kStages, ph ^= 1;
-    };
-    bool ok = true;
-    for (int k = 0; ok && next_item(k); ++k) {
-      const Item& it = item_at(k);
-      // broadcasts: known to be the same in all lanes
-      const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
-      const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
-      const bool two = __shfl_sync(0xffffffffu, it.two, 0);
-      if (lane == 0) done(k);
-      const int lead = lead_of(two, n);
-      const int clean0 = max(0, full / kKeys - lo);  // first tile with keys that not all rows see
-      // Stream 1 passes from one warp to the other, with all products of the one before
-      // complete (a commit), at the beginning and at the end of an item of two tiles.
-      // This also keeps either warp within one use of each ring stage, as the waits
-      // tell one use from the next by a parity.
-      if (role == 0) {
-        if (was_two) {
-          ok = wait_warp(&sh->mma_back, pair_ph, p.err, abort);
-          pair_ph ^= 1;
-        }
-        if (two && elect_one()) umma_commit(&sh->mma_go);
-        __syncwarp();
-      } else if (two) {
-        ok = wait_warp(&sh->mma_go, pair_ph, p.err, abort);
-        pair_ph ^= 1;
-      }
-      was_two = two;
-      // Parities of what the other warp waits for: ns tiles of stream s.
-      auto skip = [&](int s, int ns) {
-        if (ns > 0) q_ph ^= 1u << s;
-        p_ph ^= (((ns + 1) >> 1) & 1u) << (2 * s);
-        p_ph ^= ((ns >> 1) & 1u) << (2 * s + 1);
-      };
-      if (two) {
-        skip(role ^ 1, n);
-      } else if (role) {  // all of this item
-        skip(0, (n + 1) / 2);
-        skip(1, n / 2);
-        for (int j = clean0; j < n; ++j) clean_ph ^= 1u << ((st + lead + j) % kStages);
-        advance(n + lead);
-        continue;
-      }
-      // ---- the first scores
-      for (int pl = 0; ok && pl < lead; ++pl) {
-        const int s = two ? role : pl & 1, b = two ? pl : pl >> 1;
-        if (b == 0) {
-          ok = wait_warp(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
-          q_ph ^= 1u << s;
-        }
-        ok = ok && wait_warp(&sh->full[st], ph, p.err, abort);
-        tc_fence_after();
-        if (ok && elect_one()) {
-          issue_scores(s, b);
-          umma_commit(&sh->empty[st]);
-        }
-        __syncwarp();
-        advance(1);
-      }
-      // ---- P V of tile j, then the scores of tile j + lead into the same buffer
-      for (int j = 0; ok && j < n; ++j) {
-        const int s = two ? role : j & 1, i = two ? j : j >> 1, b = i & 1;
-        const int hop = two ? 1 : 2;  // to the stream's next tile
-        ok = wait_warp(&sh->full[st], ph, p.err, abort);
-        if (ok && j >= clean0) {
-          ok = wait_warp(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort);
-          clean_ph ^= 1u << st;
-        }
-        ok = ok && wait_warp(&sh->pfull[s][b], (p_ph >> (2 * s + b)) & 1, p.err, abort);
-        if (!ok) break;
-        p_ph ^= 1u << (2 * s + b);
-        tc_fence_after();
-        if (elect_one()) {
-          uint32_t d = tmem_u + 4 * kKeys + s * D, a = tmem_u + s * (2 * kKeys) + b * kKeys;
-          uint32_t vd = ring_v + st * (Sh::kStageBytes >> 4);
-          opaque(d, a, vd);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * Sh::kHalfBytes + (kk & 3) * 32) >> 4;
+              if (kk == 0)
+                mma_ss<false>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
+              else
+                mma_ss<true>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
+            }
+            umma_commit(&sh->sfull[s]);
+            if (!two || s == 1) umma_commit(&sh->empty[st]);
+          }
+          __syncwarp();
+          return true;
+        };
+        auto values = [&](int s, int i) {  // O_s += P_s V
+          const int j = two ? i : 2 * i + s;
+          const uint32_t pl = base + v_place(two, j, n);
+          const uint32_t st = pl % kStages;
+          if (!wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
+          if ((lo + j + 1) * kTile > full) {
+            if (!wait_warp(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort)) return false;
+            if (!two || s == 1) clean_ph ^= 1u << st;
+          }
+          if (!wait_warp(&sh->pfull[s], (p_ph >> s) & 1, p.err, abort)) return false;
+          p_ph ^= 1u << s;
+          tc_fence_after();
+          const uint32_t vd =
+              __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring) + st * Sh::kTileBytes, Sh::kHalfBytes), 0);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(i != 0));
-          if (j + 2 * hop <= n + hop - 1 && j + 2 * hop > n - 1) umma_commit(&sh->olast[s]);
-          if (j + hop >= n) umma_commit(&sh->ofull[s]);
-          if (j + lead < n) issue_scores(s, b);
-          umma_commit(&sh->empty[st]);
+            for (int kk = 0; kk < kTile / 16; ++kk)
+              mma_ts(tmem_u + 2 * kTile + s * D, tmem_u + s * kTile + kk * 8, vd + kk * (2048 >> 4), idesc_o,
+                     (i | kk) != 0);
+            if (!two || s == 1) umma_commit(&sh->empty[st]);
+            if (i == (s ? n1 : n0) - 1) umma_commit(&sh->ofull[s]);
+          }
+          __syncwarp();
+          return true;
+        };
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (ok && (s ? n1 : n0) > 0) {
+            ok = wait_warp(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
+            q_ph ^= 1u << s;
+            ok = ok && scores(s, 0);
+          }
+        for (int i = 0; ok && i < n0; ++i) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int mine_n = s ? n1 : n0;
+            if (ok && i < mine_n) {
+              ok = values(s, i);
+              if (ok && i + 1 < mine_n) ok = scores(s, i + 1);
+            }
+          }
         }
-        __syncwarp();
-        advance(1);
+        base += 2 * n;
       }
-      if (role == 1 && ok && elect_one()) umma_commit(&sh->mma_back);
-      __syncwarp();
+    }
+  } else if (warp == 11) {
+    // ------------------------------------------------------------ the items
+    if (lane == 0) {
+      Walk walk = sh->start;
+      for (int k = 0;; ++k) {
+        if (!wait_bar(&sh->item_empty[k % kItems], ((k / kItems) & 1) ^ 1, p.err, abort)) break;
+        Item it;
+        const bool more = walk.next(p, it);
+        if (!more) it.lo = it.hi = 0;
+        sh->items[k % kItems] = it;
+        mbar_arrive(&sh->item_full[k % kItems]);
+        if (!more) break;
+      }
     }
   } else if (warp == 10) {
-    // ------------------------------------------------------------ items; V rows that no MMA may see
-    Walk walk;
-    walk.b = sh->start_b, walk.h = 0, walk.i0 = 0, walk.off = 0;
-    walk.u = u0, walk.u1 = u1;
-    if (walk.b < p.B) {
-      walk.r = load_request(p, walk.b);
-      const int step = 2 * p.tok_tile;
-      const long long per_head = head_units(p, walk.r);
-      long long o = sh->start_u;
-      walk.h = static_cast<int>(o / per_head);
-      o -= walk.h * per_head;
-      for (;;) {
-        const int units = tiles_of(keys_needed(p, walk.r, min(walk.r.n, walk.i0 + step))) + kItemUnits;
-        if (o < units) break;
-        o -= units;
-        walk.i0 += step;
-      }
-      walk.off = static_cast<int>(o);
-    }
-    int handed = 0;         // items handed out
-    bool ended = false;
-    // Hands out what there is room for, and waits for room only for item k itself.
-    auto hand_out = [&](int k) {
-      while (!ended && handed <= k + kItems - 1) {
-        uint64_t* room = &sh->item_empty[handed % kItems];
-        const uint32_t ph = ((handed / kItems) & 1) ^ 1;
-        if (handed > k ? !mbar_test(room, ph) : !wait_bar(room, ph, p.err, abort)) break;
-        Item it;
-        ended = !walk.next(p, it);
-        if (ended) it.lo = it.hi = 0;
-        sh->items[handed % kItems] = it;
-        mbar_arrive(&sh->item_full[handed % kItems]);
-        ++handed;
-      }
-    };
-    uint32_t st = 0, ph = 0, issued_ph = 0;
+    // ------------------------------------------------------------ V rows that no MMA may see
+    uint32_t base = 0, issued_ph = 0;
     bool ok = true;
-    for (int k = 0; ok; ++k) {
-      if (lane == 0) hand_out(k);
-      __syncwarp();
-      if (!next_item(k)) break;
+    for (int k = 0; ok && next_item(k); ++k) {
       const Item it = item_at(k);
       __syncwarp();
       if (lane == 0) done(k);
-      const int n = it.hi - it.lo, lead = lead_of(it.two, n), seq = k + 1;
-      for (int pl = 0; ok && pl < n + lead; ++pl, ++st == kStages ? (st = 0, ph ^= 1) : 0) {
-        const int key0 = (it.lo + pl - lead) * kKeys;
-        if (pl < lead || key0 + kKeys <= it.full) continue;
+      const int n = it.hi - it.lo, seq = k + 1;
+      for (int j = 0; ok && j < n; ++j) {
+        const int key0 = (it.lo + j) * kTile;
+        if (key0 + kTile <= it.full) continue;
+        const uint32_t pl = base + v_place(it.two, j, n);
+        const uint32_t st = pl % kStages;
         ok = wait_warp(&sh->vissued[st], (issued_ph >> st) & 1, p.err, abort) &&
-             wait_warp(&sh->full[st], ph, p.err, abort);
+             wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort);
         if (!ok) break;
         issued_ph ^= 1u << st;
-        unsigned char* tile = ring + st * Sh::kStageBytes + Sh::kKvBytes;
+        unsigned char* tile = ring + st * Sh::kTileBytes;
         bool bad = false;
-        for (int r = lane; r < kKeys; r += 32) {
+        for (int r = lane; r < kTile; r += 32) {
           const int key = key0 + r;
           if (key < it.full) continue;
           const bool beyond = key >= it.need;
@@ -716,7 +671,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int hf = 0; hf < Sh::kHalves; ++hf) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kKvHalf + r * 128 + (((c + lane) & 7) << 4));
+              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kHalfBytes + r * 128 + (((c + lane) & 7) << 4));
               if (beyond) {
                 *at = make_uint4(0, 0, 0, 0);
                 continue;
@@ -740,15 +695,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->vclean[st]);
       }
+      base += 2 * n;
     }
   } else {
     // ------------------------------------------------------------ softmax, one thread per row
     const int s = warp >> 2;             // stream
     const int row = tid & (kTile - 1);   // row of the tile
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + s * (2 * kKeys) + lanes, to = tmem + 4 * kKeys + s * D + lanes;
-    uint32_t s_ph = 0, o_ph = 0, last_ph = 0, b_ph = 0;  // parities: S (bit buffer), O, olast, joins
-    bool o1_pending = false;                             // stream 1: stream 0 has yet to read O_1
+    const uint32_t ts = tmem + s * kTile + lanes, to = tmem + 2 * kTile + s * D + lanes;
+    uint32_t s_ph = 0, o_ph = 0, b_ph = 0;  // parities: S, O, joins
+    bool o1_pending = false;                // stream 1: stream 0 has yet to read O_1
     bool ok = true;
     const int rt = row / p.G;
 
@@ -758,15 +714,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (!x.two && s == 1 && n < 2) return;
       const int tok0 = x.i0 + (x.two ? s * p.tok_tile : 0);
       const int rows = min(p.tok_tile, x.i0 + x.ntok - tok0) * p.G;
-      constexpr int kChunks = D / 8;
+      constexpr int kChunks = D / 8, kStep = kTile / kChunks;  // a thread: one chunk of every kStep-th row
+      const int c = row % kChunks, r0 = row / kChunks;
       const uint16_t* src = p.q + static_cast<long long>(x.first + tok0) * p.q_token +
-                            static_cast<long long>(x.h) * p.G * p.q_head;
-      unsigned char* qs = smem + s * Sh::kQBytes;
-      for (int i = row; i < rows * kChunks; i += kTile) {
-        const int r = i / kChunks, c = i % kChunks;
-        const int tk = r / p.G, g = r - tk * p.G;
-        const uint4 v = ld_ro_v4(src + tk * p.q_token + g * p.q_head + c * 8);
-        *reinterpret_cast<uint4*>(qs + (c >> 3) * Sh::kQHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                            static_cast<long long>(x.h) * p.G * p.q_head + c * 8;
+      unsigned char* dst = smem + s * Sh::kTileBytes + (c >> 3) * Sh::kHalfBytes;
+      for (int rr = r0; rr < rows; rr += 8 * kStep) {  // eight loads in flight
+        uint4 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int r = rr + q * kStep, tk = r / p.G;
+          if (r < rows) v[q] = ld_ro_v4(src + tk * p.q_token + (r - tk * p.G) * p.q_head);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int r = rr + q * kStep;
+          if (r < rows) *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[q];
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -793,46 +757,47 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         o1_pending = false;
       }
       for (int i = 0; i < ns; ++i) {
-        const int j = two ? i : 2 * i + s, b = i & 1;
-        ok = wait_warp(&sh->sfull[s][b], (s_ph >> b) & 1, p.err, abort);
+        const int j = two ? i : 2 * i + s;
+        ok = wait_warp(&sh->sfull[s], s_ph, p.err, abort);
         if (!ok) break;
-        s_ph ^= 1u << b;
+        s_ph ^= 1;
         tc_fence_after();
         if (busy) {
-          const int key0 = (lo + j) * kKeys;
+          const int key0 = (lo + j) * kTile;
           const f2 scale2 = f2_make(p.scale_log2, p.scale_log2);
-          float x[kKeys];
-          uint32_t w[kKeys / 2];
-          f2 sum;
-          tmem_ld_32(ts + b * kKeys, x);
-          tmem_ld_32(ts + b * kKeys + 32, x + 32);
-          tmem_ld_wait();
-          if (key0 + kKeys > full) {
+          float x[kChunk];
+          auto read_scores = [&](int c0) {
+            tmem_ld_32(ts + c0, x);
+            tmem_ld_32(ts + c0 + 32, x + 32);
+            tmem_ld_wait();
+            if (key0 + kTile > full) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t vis = live ? visible(p, it, my_token, key0 + 32 * h) : 0u;
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t vis = live ? visible(p, it, my_token, key0 + c0 + 32 * h) : 0u;
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!((vis >> c) & 1)) x[32 * h + c] = -INFINITY;
+                for (int c = 0; c < 32; ++c)
+                  if (!((vis >> c) & 1)) x[32 * h + c] = -INFINITY;
+              }
             }
-          }
-          float mx[4] = {x[0], x[1], x[2], x[3]};
+          };
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c0 = kTile - kChunk; c0 >= 0; c0 -= kChunk) {  // ends with the first chunk in x
+            read_scores(c0);
+            float mx[4] = {top, x[1], x[2], x[3]};
+            mx[0] = fmaxf(mx[0], x[0]);
 #pragma unroll
-          for (int c = 4; c < kKeys; c += 8) {
+            for (int c = 4; c < kChunk; c += 8) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              mx[q] = c + 4 + q < kKeys ? fmaxf(fmaxf(mx[q], x[c + q]), x[c + 4 + q]) : fmaxf(mx[q], x[c + q]);
+              for (int q = 0; q < 4; ++q)
+                mx[q] = c + 4 + q < kChunk ? fmaxf(fmaxf(mx[q], x[c + q]), x[c + 4 + q]) : fmaxf(mx[q], x[c + q]);
+            }
+            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          top *= p.scale_log2;
           if (i == 0) {
             m = top;
           } else if (const bool raise = live && top > m + kRaise; __any_sync(0xffffffffu, raise)) {
-            // O must hold all tiles before this one: the next scores were issued after P V
-            // of the tile before; at the last tile olast says so.
-            ok = i + 1 < ns ? wait_warp(&sh->sfull[s][b ^ 1], (s_ph >> (b ^ 1)) & 1, p.err, abort)
-                            : wait_warp(&sh->olast[s], last_ph, p.err, abort);
-            if (!ok) break;
-            tc_fence_after();
             // each row by its own values alone, whatever the rows beside it do
             const float f = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx(m - top);
             m = raise ? top : m;
@@ -850,26 +815,32 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const float base = m == -INFINITY ? 0.f : -m;
           const f2 base2 = f2_make(base, base);
           f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+          // P of the first chunk goes over scores 0 .. 31, of the second over 32 .. 63: both
+          // already read.
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTile; c0 += kChunk) {
+            if (c0) read_scores(c0);
+            uint32_t w[kChunk / 2];
 #pragma unroll
-          for (int q = 0; q < kKeys / 2; ++q) {
-            float a, c;
-            f2_split(f2_fma(f2_make(x[2 * q], x[2 * q + 1]), scale2, base2), a, c);
-            a = exp2_approx(a);
-            c = exp2_approx(c);
-            sums[q & 1] = f2_add(sums[q & 1], f2_make(a, c));
-            w[q] = pack_pair<BF16>(a, c);
+            for (int q = 0; q < kChunk / 2; ++q) {
+              float a, c;
+              f2_split(f2_fma(f2_make(x[2 * q], x[2 * q + 1]), scale2, base2), a, c);
+              a = exp2_approx(a);
+              c = exp2_approx(c);
+              sums[q & 1] = f2_add(sums[q & 1], f2_make(a, c));
+              w[q] = pack_pair<BF16>(a, c);
+            }
+            tmem_st_16(ts + c0 / 2, w);
+            tmem_st_16(ts + c0 / 2 + 16, w + 16);
           }
-          tmem_st_16(ts + b * kKeys, w);
-          tmem_st_16(ts + b * kKeys + 16, w + 16);
-          sum = f2_add(sums[0], sums[1]);
           float a, c;
-          f2_split(sum, a, c);
+          f2_split(f2_add(sums[0], sums[1]), a, c);
           l += a + c;
           tmem_st_wait();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->pfull[s][b]);
+        if (lane == 0) mbar_arrive(&sh->pfull[s]);
       }
       if (!ok) break;
       more = next_item(k + 1);
@@ -893,7 +864,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       ok = wait_warp(&sh->ofull[s], o_ph, p.err, abort);
       if (!ok) break;
       o_ph ^= 1;
-      if (ns > 1) last_ph ^= 1;  // (completed before ofull)
       if (joined && s == 1) {
         sh->m1[row] = m;
         sh->l1[row] = l;
@@ -942,7 +912,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             for (int q = 0; q < 32; ++q) o[q] *= f0;
           }
           if (bad && live) {  // values that were kept out of the MMA
-            for (int key = max(full, lo * kKeys); key < min(it.need, it.hi * kKeys); ++key) {
+            for (int key = max(full, lo * kTile); key < min(it.need, it.hi * kTile); ++key) {
               if (!(visible(p, it, my_token, key) & 1)) continue;
               const int page = p.table[static_cast<long long>(it.b) * p.table_stride + (key >> p.page_shift)];
               if (page < 0 || page >= p.num_pages) continue;
@@ -1075,7 +1045,7 @@ int make_cache_map(const void* base, const CacheStrides& cs, int D, int rows, in
                               static_cast<cuuint64_t>(Hkv), static_cast<cuuint64_t>(pages)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(cs.row) * 2, static_cast<cuuint64_t>(cs.head) * 2,
                                  static_cast<cuuint64_t>(cs.page) * 2};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kKeys)), 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kTile)), 1, 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1149,7 +1119,7 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
                        static_cast<const uint16_t*>(v_cache), cs, block_table, table_stride, table_width, kv_lens,
                        cu_new, reinterpret_cast<const unsigned long long*>(mask), mask_words,
                        static_cast<uint16_t*>(out), lse, B, T, Hq, Hkv, G, kTile / G, num_pages,
-                       log2_of(page_size), kMinUnits, scale * 1.4426950408889634f,
+                       log2_of(page_size), scale * 1.4426950408889634f,
                        reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kMetaBytes),
                        static_cast<Meta*>(workspace), dev.err};
   auto st = static_cast<cudaStream_t>(stream);
