@@ -7,25 +7,24 @@
 // The query heads that share a KV head are rows of one tile: row r of a tile is
 // token r / G, head r % G (G = Hq / Hkv), so K and V are read once for all of them
 // and a tile of 128 rows holds 128 / G tokens.  A work item is (request, KV head,
-// two tiles of tokens); its keys come in tiles of 128.
+// one tile of tokens); its keys come in tiles of 64.
 //
-// One persistent CTA per SM, warp-specialised:
-//   warps 0-7, 8-15 softmax of stream 0 and stream 1: two threads per row, 64 keys each
-//   warp 16         TMA: the pages of a K or V tile into a ring of stages, one lane per
-//                   page and 64-value half, 128-byte swizzle
-//   warp 17         tcgen05.mma: S_s = Q_s K^T (128 x 128, both operands from shared
-//                   memory), O_s += P_s V (P_s from tensor memory)
-//   warp 18         tensor-memory allocation; rows of V that no MMA may see (below)
-//   warp 19         walks this CTA's share of the work and hands out its items
-// The two streams hide each other's softmax: while one is in its exponentials the
-// tensor core works for the other.  With two tiles of tokens both streams go
-// through every key tile (which is loaded once); with one tile they take the even
-// and the odd key tiles, each with a softmax state of its own, and stream 0 joins
-// the two at the end.  Tensor memory: S_0, S_1 (128 columns each; P_s is written over S_s), O_0,
-// O_1 (D each).
+// Two persistent CTAs per SM, each warp-specialised:
+//   warps 0-3  softmax, one thread per row
+//   warp 4     TMA: the pages of a K or V tile into a ring of stages, one lane per
+//              page and 64-value half, 128-byte swizzle
+//   warp 5     tcgen05.mma: S = Q K^T (128 x 64, both operands from shared
+//              memory), O += P V (P from tensor memory)
+//   warp 6     tensor-memory allocation; rows of V that no MMA may see (below)
+//   warp 7     walks this CTA's share of the work and hands out its items
+// Tensor memory: two buffers of scores (64 columns each; P is written over the
+// scores it comes from) and O (D columns).  While the softmax has one tile of scores
+// the tensor core computes the next one into the other buffer.  The two CTAs
+// of an SM hide each other's waits: while one is between two items (its last product,
+// the output, the next Q) the other keeps the memory and the tensor core busy.
 //
 // Work is split evenly over the CTAs: every CTA adds up the key tiles of all items
-// (from the lengths, on the GPU; an item counts one more for its fixed cost) and
+// (from the lengths, on the GPU; an item counts kItemUnits more for its fixed cost) and
 // takes its share of the line, which may begin and end inside an item.  An item
 // that lies in several CTAs is written as unnormalised fp32 partials with their
 // maxima and sums, which a second small kernel joins in CTA order.
@@ -51,15 +50,14 @@
 namespace ngb {
 namespace {
 
-constexpr int kTile = 128;         // rows of a query tile, keys of a key tile
-constexpr int kAttnThreads = 384;  // 12 warps
-constexpr int kChunk = 64;         // scores that a softmax thread holds at a time
-constexpr int kRowsMax = 2 * kTile;
+constexpr int kTile = 128;         // rows of a query tile
+constexpr int kKeys = 64;          // keys of a key tile
+constexpr int kAttnThreads = 256;  // 8 warps, two CTAs an SM
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
 constexpr int kBadSlots = 8;
 constexpr int kItems = 4;          // work items handed out ahead
-constexpr int kMinUnits = 4;       // least work of a CTA, in key tiles
-constexpr int kItemUnits = 1;      // what an item costs beside its key tiles, in key tiles
+constexpr int kMinUnits = 8;       // least work of a CTA, in key tiles
+constexpr int kItemUnits = 2;      // what an item costs beside its key tiles, in key tiles
 
 // A work item as one CTA sees it.
 struct alignas(16) Item {
@@ -67,19 +65,17 @@ struct alignas(16) Item {
   int first, ctx, kv;    // the request's first token row, rows before its new tokens, all rows
   int need, full;        // keys that the item's tokens need; leading ones that all of them see
   int nt, lo, hi;        // key tiles of the item; this CTA's are [lo, hi); none: the end of the work
-  int two;               // two tiles of tokens
-  int pad[3];
 };
 
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kTileBytes = kTile * D * 2;           // a Q, K or V tile
-  static constexpr int kHalfBytes = kTile * 128;             // its 64-value half
-  static constexpr int kStages = D == 128 ? 5 : 10;          // ring: 160 KB
-  static constexpr int kSmem = (2 + kStages) * kTileBytes;
-  // One partial: kRowsMax rows of D values, maxima, sums.
-  static constexpr size_t kPartFloats = static_cast<size_t>(kRowsMax) * (D + 2);
+  static constexpr int kQBytes = kTile * D * 2, kQHalf = kTile * 128;   // a Q tile, its 64-value half
+  static constexpr int kKvBytes = kKeys * D * 2, kKvHalf = kKeys * 128; // a K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 10;                     // ring: 80 KB
+  static constexpr int kSmem = kQBytes + kStages * kKvBytes;
+  // One partial: 128 rows of D values, maxima, sums.
+  static constexpr size_t kPartFloats = static_cast<size_t>(kTile) * (D + 2);
 };
 
 // What the joining kernel needs to know of a CTA.
@@ -139,11 +135,11 @@ __device__ __forceinline__ int keys_needed(const TreeAttnArgs& p, const Request&
 __device__ __forceinline__ int keys_full(const TreeAttnArgs& p, const Request& r, int i0) {
   return p.mask ? r.ctx : min(r.kv, r.ctx + i0 + 1);
 }
-__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kKeys - 1) / kKeys); }
 
 // Units of one KV head of a request: its tiles, and kItemUnits for each item.
 __device__ __forceinline__ long long head_units(const TreeAttnArgs& p, const Request& r) {
-  const int step = 2 * p.tok_tile;
+  const int step = p.tok_tile;
   if (p.mask) return static_cast<long long>((r.n + step - 1) / step) * (tiles_of(r.kv) + kItemUnits);
   long long u = 0;
   for (int i0 = 0; i0 < r.n; i0 += step) u += tiles_of(keys_needed(p, r, min(r.n, i0 + step))) + kItemUnits;
@@ -165,7 +161,7 @@ struct Walk {
   Request r;
 
   __device__ __forceinline__ bool next(const TreeAttnArgs& p, Item& it) {
-    const int step = 2 * p.tok_tile;
+    const int step = p.tok_tile;
     while (u < u1 && b < p.B) {
       if (!loaded) r = load_request(p, b);
       loaded = 1;
@@ -181,7 +177,6 @@ struct Walk {
       it.b = b, it.h = h, it.i0 = i0, it.ntok = i1 - i0;
       it.first = r.first, it.ctx = r.ctx, it.kv = r.kv, it.need = need, it.full = keys_full(p, r, i0);
       it.nt = nt, it.lo = max(0, off - kItemUnits), it.hi = off + take - kItemUnits;
-      it.two = it.ntok > p.tok_tile;
       u += take;
       off += take;
       if (off == nt + kItemUnits) {
@@ -205,16 +200,15 @@ struct Walk {
 template <int kStages>
 struct alignas(16) Shared {
   uint64_t full[kStages], empty[kStages], vissued[kStages], vclean[kStages];
-  uint64_t qfull[2], sfull[2], pfull[2], ofull[2];
-  uint64_t ml1, o1read;
+  uint64_t sfull[2], pfull[2];  // by buffer
+  uint64_t qfull, ofull, olast; // olast: all but the last P V of an item are done
   uint64_t item_full[kItems], item_empty[kItems];
   Item items[kItems];
   long long warp_sum[kAttnThreads / 32];
-  Walk start;                        // where this CTA's share begins
+  Walk start;                   // where this CTA's share begins
   uint32_t tmem;
   int abort;
   int bad[kBadSlots];
-  float m1[kTile], l1[kTile];        // stream 1's maxima and sums, for stream 0
 };
 
 // ---------------------------------------------------------------------------
@@ -255,14 +249,19 @@ __device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr, uint32_t half_byt
   return (addr >> 4) | ((half_bytes >> 4) << 16);
 }
 
+// Keeps the compiler from computing the operands of all products of an item ahead
+// of its loop, which takes more registers than the warp has.
+__device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b, uint32_t& c) {
+  asm volatile("" : "+r"(a), "+r"(b), "+r"(c));
+}
+
 // D[tmem] (+)= A * B, descriptors by their low words; A from shared / from tensor memory.
-template <bool kAccumulate>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .b64 x, y;\n\t.reg .pred p;\n\t"
       "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "n"(kAccumulate ? 1 : 0)
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -340,13 +339,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, unsign
   return __all_sync(0xffffffffu, wait_bar(bar, parity, err, abort));
 }
 
-// Place of key tile j (of n) in the order in which the tiles are loaded: with two
-// query tiles K0 V0 K1 V1 ..., with one K0 K1 V0 K2 V1 ... (the order of the MMAs).
-__device__ __forceinline__ int k_place(bool two, int j) { return two ? 2 * j : (j ? 2 * j - 1 : 0); }
-__device__ __forceinline__ int v_place(bool two, int j, int n) {
-  return two ? 2 * j + 1 : (j == n - 1 ? 2 * n - 1 : 2 * j + 2);
-}
-
 // 32 bits of token row `row`'s mask from bit `at` on (which may be negative).
 __device__ __forceinline__ uint32_t mask_window(const TreeAttnArgs& p, int row, int at) {
   if (at <= -32) return 0;
@@ -370,13 +362,13 @@ __device__ __forceinline__ uint32_t visible(const TreeAttnArgs& p, const Item& i
 // Main kernel
 // ---------------------------------------------------------------------------
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kAttnThreads, 2)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                      const __grid_constant__ TreeAttnArgs p) {
   using Sh = Shape<D>;
   constexpr int kStages = Sh::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];  // 1024: the swizzle atom
-  unsigned char* ring = smem + 2 * Sh::kTileBytes;  // after Q_0, Q_1
+  unsigned char* ring = smem + Sh::kQBytes;
   auto* sh = reinterpret_cast<Shared<kStages>*>(smem + Sh::kSmem);
   volatile int* abort = &sh->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -388,18 +380,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&sh->vissued[s], 1);
       mbar_init(&sh->vclean[s], 1);
     }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->sfull[b], 1);
+      mbar_init(&sh->pfull[b], 4);
+    }
+    mbar_init(&sh->qfull, 4);
+    mbar_init(&sh->ofull, 1);
+    mbar_init(&sh->olast, 1);
     for (int s = 0; s < kItems; ++s) {
       mbar_init(&sh->item_full[s], 1);
-      mbar_init(&sh->item_empty[s], 11);  // TMA, MMA, V rows, 8 softmax warps
+      mbar_init(&sh->item_empty[s], 7);  // TMA, MMA, V rows, 4 softmax warps
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&sh->qfull[s], 4);
-      mbar_init(&sh->sfull[s], 1);
-      mbar_init(&sh->pfull[s], 4);
-      mbar_init(&sh->ofull[s], 1);
-    }
-    mbar_init(&sh->ml1, 4);
-    mbar_init(&sh->o1read, 4);
     sh->abort = 0;
     sh->start.u = sh->start.u1 = 0;  // no work, unless a thread finds some below
     for (int i = 0; i < kBadSlots; ++i) sh->bad[i] = 0;
@@ -407,7 +398,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
-  if (warp == 10) tmem_alloc(&sh->tmem, 512);
+  if (warp == 6) tmem_alloc(&sh->tmem, 256);
   pdl_launch_next();
   pdl_wait_previous();
 
@@ -456,7 +447,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     w.r = req;
     w.h = static_cast<int>(quotient(o, hu));
     o -= w.h * hu;
-    const int step = 2 * p.tok_tile;
+    const int step = p.tok_tile;
     w.i0 = 0;
     for (;;) {
       const int units = tiles_of(keys_needed(p, req, min(req.n, w.i0 + step))) + kItemUnits;
@@ -485,15 +476,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   };
   auto done = [&](int k) { mbar_arrive(&sh->item_empty[k % kItems]); };
 
-  if (warp == 8) {
+  // Places of the ring in an item of n tiles: K0 K1 V0 K2 V1 K3 ..., the order of the MMAs.
+  if (warp == 4) {
     // ------------------------------------------------------------ TMA producer
-    const int shift = min(p.page_shift, 7);         // rows of a piece: a page, or a whole tile of one
-    const int pieces = kTile >> shift;
+    const int shift = min(p.page_shift, 6);  // rows of a piece: a page, or a whole tile of one
+    const int pieces = kKeys >> shift;
     const int piece = lane % pieces, half = lane / pieces;
     const uint32_t piece_bytes = 128u << shift;
-    const uint32_t offset = half * Sh::kHalfBytes + piece * piece_bytes;
+    const uint32_t offset = half * Sh::kKvHalf + piece * piece_bytes;
     const int page_mask = (1 << p.page_shift) - 1;
-    uint32_t it_count = 0;
+    uint32_t st = 0, ph = 0;  // stage and parity of the next place
     bool ok = true;
     for (int k = 0; ok && next_item(k); ++k) {
       const Item it = item_at(k);
@@ -501,24 +493,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (lane == 0) done(k);
       const int n = it.hi - it.lo;
       const int* row = p.table + static_cast<long long>(it.b) * p.table_stride;
-      auto active_at = [&](int j) {
-        return half < Sh::kHalves && (it.lo + j) * kTile + (piece << shift) < it.need;
-      };
-      auto page_at = [&](int j) -> int {
-        if (j >= n || !active_at(j)) return 0;
-        return row[((it.lo + j) * kTile + (piece << shift)) >> p.page_shift];
-      };
+      auto key_at = [&](int j) { return (it.lo + j) * kKeys + (piece << shift); };
+      auto active_at = [&](int j) { return half < Sh::kHalves && j < n && key_at(j) < it.need; };
+      auto page_at = [&](int j) { return active_at(j) ? row[key_at(j) >> p.page_shift] : 0; };
       auto load = [&](bool is_v, int j, int page) {
-        const uint32_t s = it_count % kStages, ph = (it_count / kStages) & 1;
-        ++it_count;
-        if (!wait_warp(&sh->empty[s], ph ^ 1, p.err, abort)) return false;
+        if (!wait_warp(&sh->empty[st], ph ^ 1, p.err, abort)) return false;
         const bool active = active_at(j);
         const unsigned votes = __ballot_sync(0xffffffffu, active);
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->full[s], __popc(votes) * piece_bytes);
-          // From here on the parity of full[s] means this use to the V-row warp, which
+          mbar_arrive_expect_tx(&sh->full[st], __popc(votes) * piece_bytes);
+          // From here on the parity of full[st] means this use to the V-row warp, which
           // only looks at some uses and could take another for it.
-          if (is_v && (it.lo + j + 1) * kTile > it.full) mbar_arrive(&sh->vissued[s]);
+          if (is_v && (it.lo + j + 1) * kKeys > it.full) mbar_arrive(&sh->vissued[st]);
         }
         __syncwarp();
         if (active) {
@@ -526,110 +512,90 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             atomicOr(p.err, kErrBadIndex);
             page = p.num_pages;
           }
-          const int r = ((it.lo + j) * kTile + (piece << shift)) & page_mask;
-          tma_load_4d(smem_u32(ring + s * Sh::kTileBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[s],
-                      half * 64, r, it.h, page);
+          tma_load_4d(smem_u32(ring + st * Sh::kKvBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[st],
+                      half * 64, key_at(j) & page_mask, it.h, page);
         }
+        if (++st == kStages) st = 0, ph ^= 1;
         return true;
       };
-      const int lag = it.two ? 0 : 1;
-      int pg = page_at(0), pg_prev = 0;
-      for (int j = 0; ok && j < n + lag; ++j) {
-        const int pg_next = page_at(j + 1);
-        if (j < n) ok = load(false, j, pg);
-        if (ok && j >= lag) ok = load(true, j - lag, lag ? pg_prev : pg);
-        pg_prev = pg;
-        pg = pg_next;
+      int pg0 = page_at(0), pg1 = page_at(1);  // of tiles j and j + 1
+      ok = load(false, 0, pg0) && (n == 1 || load(false, 1, pg1));
+      for (int j = 0; ok && j < n; ++j) {
+        const int pg2 = page_at(j + 2);
+        ok = load(true, j, pg0) && (j + 2 >= n || load(false, j + 2, pg2));
+        pg0 = pg1;
+        pg1 = pg2;
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issuer
-    {
-      constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kTile);
-      constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
-      uint32_t base = 0;       // ring places used by earlier items
-      uint32_t clean_ph = 0;   // per stage: parity of its next cleaned use
-      uint32_t q_ph = 0, p_ph = 0;  // parities, bit s
-      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
-      bool ok = true;
-      for (int k = 0; ok && next_item(k); ++k) {
-        const Item& it = item_at(k);
-        // broadcasts: known to be the same in all lanes
-        const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
-        const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
-        const bool two = __shfl_sync(0xffffffffu, it.two, 0);
-        if (lane == 0) done(k);
-        const int n0 = two ? n : (n + 1) / 2, n1 = two ? n : n / 2;
-        auto scores = [&](int s, int i) {  // S_s = Q_s K^T of the stream's i-th tile
-          const int j = two ? i : 2 * i + s;
-          const uint32_t pl = base + k_place(two, j);
-          const uint32_t st = pl % kStages;
-          if (!wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
-          tc_fence_after();
-          const uint32_t qd = q_desc + s * (Sh::kTileBytes >> 4);
-          const uint32_t kd = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring) + st * Sh::kTileBytes), 0);
-          if (elect_one()) {
+    constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kKeys);
+    constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
+    uint32_t st = 0, ph = 0;      // stage and parity of the next place
+    uint32_t clean_ph = 0;        // per stage: parity of its next cleaned use
+    uint32_t q_ph = 0, p_ph = 0;  // parities of Q and of P (bit buffer)
+    // broadcasts: known to be the same in all lanes
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
+    const uint32_t ring_k = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring)), 0);
+    const uint32_t ring_v = __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring), Sh::kKvHalf), 0);
+    auto advance = [&]() {
+      if (++st == kStages) st = 0, ph ^= 1;
+    };
+    auto scores = [&](int b) {  // S = Q K^T into buffer b, K at the current place
+      if (!wait_warp(&sh->full[st], ph, p.err, abort)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        uint32_t d = tmem_u + b * kKeys, qd = q_desc, kd = ring_k + st * (Sh::kKvBytes >> 4);
+        opaque(d, qd, kd);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t o = ((kk >> 2) * Sh::kHalfBytes + (kk & 3) * 32) >> 4;
-              if (kk == 0)
-                mma_ss<false>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
-              else
-                mma_ss<true>(tmem_u + s * kTile, qd + o, kd + o, idesc_s);
-            }
-            umma_commit(&sh->sfull[s]);
-            if (!two || s == 1) umma_commit(&sh->empty[st]);
-          }
-          __syncwarp();
-          return true;
-        };
-        auto values = [&](int s, int i) {  // O_s += P_s V
-          const int j = two ? i : 2 * i + s;
-          const uint32_t pl = base + v_place(two, j, n);
-          const uint32_t st = pl % kStages;
-          if (!wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort)) return false;
-          if ((lo + j + 1) * kTile > full) {
-            if (!wait_warp(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort)) return false;
-            if (!two || s == 1) clean_ph ^= 1u << st;
-          }
-          if (!wait_warp(&sh->pfull[s], (p_ph >> s) & 1, p.err, abort)) return false;
-          p_ph ^= 1u << s;
-          tc_fence_after();
-          const uint32_t vd =
-              __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring) + st * Sh::kTileBytes, Sh::kHalfBytes), 0);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < kTile / 16; ++kk)
-              mma_ts(tmem_u + 2 * kTile + s * D, tmem_u + s * kTile + kk * 8, vd + kk * (2048 >> 4), idesc_o,
-                     (i | kk) != 0);
-            if (!two || s == 1) umma_commit(&sh->empty[st]);
-            if (i == (s ? n1 : n0) - 1) umma_commit(&sh->ofull[s]);
-          }
-          __syncwarp();
-          return true;
-        };
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-          if (ok && (s ? n1 : n0) > 0) {
-            ok = wait_warp(&sh->qfull[s], (q_ph >> s) & 1, p.err, abort);
-            q_ph ^= 1u << s;
-            ok = ok && scores(s, 0);
-          }
-        for (int i = 0; ok && i < n0; ++i) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const int mine_n = s ? n1 : n0;
-            if (ok && i < mine_n) {
-              ok = values(s, i);
-              if (ok && i + 1 < mine_n) ok = scores(s, i + 1);
-            }
-          }
+        for (int kk = 0; kk < D / 16; ++kk)
+          mma_ss(d, qd + (((kk >> 2) * Sh::kQHalf + (kk & 3) * 32) >> 4),
+                 kd + (((kk >> 2) * Sh::kKvHalf + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+        umma_commit(&sh->sfull[b]);
+        umma_commit(&sh->empty[st]);
+      }
+      __syncwarp();
+      advance();
+      return true;
+    };
+    bool ok = true;
+    for (int k = 0; ok && next_item(k); ++k) {
+      const Item& it = item_at(k);
+      const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
+      const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
+      if (lane == 0) done(k);
+      const int clean0 = max(0, full / kKeys - lo);  // first tile with keys that not all rows see
+      ok = wait_warp(&sh->qfull, q_ph, p.err, abort);
+      q_ph ^= 1;
+      ok = ok && scores(0) && (n == 1 || scores(1));
+      for (int j = 0; ok && j < n; ++j) {  // O += P V of tile j, then the scores of tile j + 2
+        const int b = j & 1;
+        ok = wait_warp(&sh->full[st], ph, p.err, abort);
+        if (ok && j >= clean0) {
+          ok = wait_warp(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort);
+          clean_ph ^= 1u << st;
         }
-        base += 2 * n;
+        ok = ok && wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort);
+        if (!ok) break;
+        p_ph ^= 1u << b;
+        tc_fence_after();
+        if (elect_one()) {
+          uint32_t d = tmem_u + 2 * kKeys, a = tmem_u + b * kKeys, vd = ring_v + st * (Sh::kKvBytes >> 4);
+          opaque(d, a, vd);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            mma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(j != 0));
+          umma_commit(&sh->empty[st]);
+          if (j == n - 2) umma_commit(&sh->olast);
+          if (j == n - 1) umma_commit(&sh->ofull);
+        }
+        __syncwarp();
+        advance();
+        if (j + 2 < n) ok = scores(b);
       }
     }
-  } else if (warp == 11) {
+  } else if (warp == 7) {
     // ------------------------------------------------------------ the items
     if (lane == 0) {
       Walk walk = sh->start;
@@ -643,27 +609,25 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!more) break;
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == 6) {
     // ------------------------------------------------------------ V rows that no MMA may see
-    uint32_t base = 0, issued_ph = 0;
+    uint32_t place = 0, issued_ph = 0;
     bool ok = true;
     for (int k = 0; ok && next_item(k); ++k) {
       const Item it = item_at(k);
       __syncwarp();
       if (lane == 0) done(k);
       const int n = it.hi - it.lo, seq = k + 1;
-      for (int j = 0; ok && j < n; ++j) {
-        const int key0 = (it.lo + j) * kTile;
-        if (key0 + kTile <= it.full) continue;
-        const uint32_t pl = base + v_place(it.two, j, n);
-        const uint32_t st = pl % kStages;
+      for (int j = max(0, it.full / kKeys - it.lo); ok && j < n; ++j) {
+        const int key0 = (it.lo + j) * kKeys;
+        const uint32_t pl = place + min(n, j + 2) + j, st = pl % kStages;
         ok = wait_warp(&sh->vissued[st], (issued_ph >> st) & 1, p.err, abort) &&
              wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort);
         if (!ok) break;
         issued_ph ^= 1u << st;
-        unsigned char* tile = ring + st * Sh::kTileBytes;
+        unsigned char* tile = ring + st * Sh::kKvBytes;
         bool bad = false;
-        for (int r = lane; r < kTile; r += 32) {
+        for (int r = lane; r < kKeys; r += 32) {
           const int key = key0 + r;
           if (key < it.full) continue;
           const bool beyond = key >= it.need;
@@ -671,7 +635,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int hf = 0; hf < Sh::kHalves; ++hf) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kHalfBytes + r * 128 + (((c + lane) & 7) << 4));
+              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kKvHalf + r * 128 + (((c + lane) & 7) << 4));
               if (beyond) {
                 *at = make_uint4(0, 0, 0, 0);
                 continue;
@@ -695,30 +659,25 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->vclean[st]);
       }
-      base += 2 * n;
+      place += 2 * n;
     }
   } else {
     // ------------------------------------------------------------ softmax, one thread per row
-    const int s = warp >> 2;             // stream
     const int row = tid & (kTile - 1);   // row of the tile
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + s * kTile + lanes, to = tmem + 2 * kTile + s * D + lanes;
-    uint32_t s_ph = 0, o_ph = 0, b_ph = 0;  // parities: S, O, joins
-    bool o1_pending = false;                // stream 1: stream 0 has yet to read O_1
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t ts = tmem + lanes, to = tmem + 2 * kKeys + lanes;  // scores, O
+    uint32_t s_ph = 0, o_ph = 0, last_ph = 0;  // parities: S (bit buffer), O, olast
     bool ok = true;
     const int rt = row / p.G;
 
-    // Q rows of this stream's tile into shared memory (128-byte swizzle).
+    // The item's Q rows into shared memory (128-byte swizzle).
     auto load_q = [&](const Item& x) {
-      const int n = x.hi - x.lo;
-      if (!x.two && s == 1 && n < 2) return;
-      const int tok0 = x.i0 + (x.two ? s * p.tok_tile : 0);
-      const int rows = min(p.tok_tile, x.i0 + x.ntok - tok0) * p.G;
+      const int rows = x.ntok * p.G;
       constexpr int kChunks = D / 8, kStep = kTile / kChunks;  // a thread: one chunk of every kStep-th row
       const int c = row % kChunks, r0 = row / kChunks;
-      const uint16_t* src = p.q + static_cast<long long>(x.first + tok0) * p.q_token +
+      const uint16_t* src = p.q + static_cast<long long>(x.first + x.i0) * p.q_token +
                             static_cast<long long>(x.h) * p.G * p.q_head + c * 8;
-      unsigned char* dst = smem + s * Sh::kTileBytes + (c >> 3) * Sh::kHalfBytes;
+      unsigned char* dst = smem + (c >> 3) * Sh::kQHalf;
       for (int rr = r0; rr < rows; rr += 8 * kStep) {  // eight loads in flight
         uint4 v[8];
 #pragma unroll
@@ -734,70 +693,61 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->qfull[s]);
+      if (lane == 0) mbar_arrive(&sh->qfull);
     };
 
     bool more = next_item(0);
     if (more) load_q(item_at(0));
-    int meta_tail = 0, meta_ends = 0, meta_token = 0, meta_ntok = 0, meta_head = 0;
+    if (tid == 0) p.meta[blockIdx.x] = Meta{};
     for (int k = 0; more; ++k) {
       const Item& it = item_at(k);
-      const bool two = it.two;
       const int n = it.hi - it.lo, lo = it.lo, full = it.full;
-      const int ns = two ? n : (n + 1 - s) / 2;
-      const int tok0 = it.i0 + (two ? s * p.tok_tile : 0);
-      const int rows = min(p.tok_tile, it.i0 + it.ntok - tok0) * p.G;
-      const bool busy = (warp & 3) * 32 < rows;  // this warp has rows
+      const int rows = it.ntok * p.G;
+      const bool busy = warp * 32 < rows;  // this warp has rows
       const bool live = row < rows;
-      const int my_token = tok0 + (live ? rt : 0);
+      const int my_token = it.i0 + (live ? rt : 0);
       float m = -INFINITY, l = 0.f;
-      if (o1_pending && ns > 0) {  // stream 0 must have read O_1, m1 and l1 of an item before
-        ok = wait_warp(&sh->o1read, b_ph ^ 1, p.err, abort);
+      for (int j = 0; j < n; ++j) {
+        const int b = j & 1;
+        ok = wait_warp(&sh->sfull[b], (s_ph >> b) & 1, p.err, abort);
         if (!ok) break;
-        o1_pending = false;
-      }
-      for (int i = 0; i < ns; ++i) {
-        const int j = two ? i : 2 * i + s;
-        ok = wait_warp(&sh->sfull[s], s_ph, p.err, abort);
-        if (!ok) break;
-        s_ph ^= 1;
+        s_ph ^= 1u << b;
         tc_fence_after();
         if (busy) {
-          const int key0 = (lo + j) * kTile;
+          const int key0 = (lo + j) * kKeys;
           const f2 scale2 = f2_make(p.scale_log2, p.scale_log2);
-          float x[kChunk];
-          auto read_scores = [&](int c0) {
-            tmem_ld_32(ts + c0, x);
-            tmem_ld_32(ts + c0 + 32, x + 32);
-            tmem_ld_wait();
-            if (key0 + kTile > full) {
+          float x[kKeys];
+          uint32_t w[kKeys / 2];
+          f2 sum;
+          tmem_ld_32(ts + b * kKeys, x);
+          tmem_ld_32(ts + b * kKeys + 32, x + 32);
+          tmem_ld_wait();
+          if (key0 + kKeys > full) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t vis = live ? visible(p, it, my_token, key0 + c0 + 32 * h) : 0u;
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t vis = live ? visible(p, it, my_token, key0 + 32 * h) : 0u;
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
-                  if (!((vis >> c) & 1)) x[32 * h + c] = -INFINITY;
-              }
+              for (int c = 0; c < 32; ++c)
+                if (!((vis >> c) & 1)) x[32 * h + c] = -INFINITY;
             }
-          };
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c0 = kTile - kChunk; c0 >= 0; c0 -= kChunk) {  // ends with the first chunk in x
-            read_scores(c0);
-            float mx[4] = {top, x[1], x[2], x[3]};
-            mx[0] = fmaxf(mx[0], x[0]);
-#pragma unroll
-            for (int c = 4; c < kChunk; c += 8) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                mx[q] = c + 4 + q < kChunk ? fmaxf(fmaxf(mx[q], x[c + q]), x[c + 4 + q]) : fmaxf(mx[q], x[c + q]);
-            }
-            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           }
-          top *= p.scale_log2;
-          if (i == 0) {
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int c = 4; c < kKeys; c += 8) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mx[q] = c + 4 + q < kKeys ? fmaxf(fmaxf(mx[q], x[c + q]), x[c + 4 + q]) : fmaxf(mx[q], x[c + q]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          if (j == 0) {
             m = top;
           } else if (const bool raise = live && top > m + kRaise; __any_sync(0xffffffffu, raise)) {
+            // O must hold all tiles before this one: the next scores were issued after P V
+            // of the tile before; at the last tile olast says so.
+            ok = j + 1 < n ? wait_warp(&sh->sfull[b ^ 1], (s_ph >> (b ^ 1)) & 1, p.err, abort)
+                            : wait_warp(&sh->olast, last_ph, p.err, abort);
+            if (!ok) break;
+            tc_fence_after();
             // each row by its own values alone, whatever the rows beside it do
             const float f = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_approx(m - top);
             m = raise ? top : m;
@@ -815,104 +765,60 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const float base = m == -INFINITY ? 0.f : -m;
           const f2 base2 = f2_make(base, base);
           f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
-          // P of the first chunk goes over scores 0 .. 31, of the second over 32 .. 63: both
-          // already read.
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += kChunk) {
-            if (c0) read_scores(c0);
-            uint32_t w[kChunk / 2];
 #pragma unroll
-            for (int q = 0; q < kChunk / 2; ++q) {
-              float a, c;
-              f2_split(f2_fma(f2_make(x[2 * q], x[2 * q + 1]), scale2, base2), a, c);
-              a = exp2_approx(a);
-              c = exp2_approx(c);
-              sums[q & 1] = f2_add(sums[q & 1], f2_make(a, c));
-              w[q] = pack_pair<BF16>(a, c);
-            }
-            tmem_st_16(ts + c0 / 2, w);
-            tmem_st_16(ts + c0 / 2 + 16, w + 16);
+          for (int q = 0; q < kKeys / 2; ++q) {
+            float a, c;
+            f2_split(f2_fma(f2_make(x[2 * q], x[2 * q + 1]), scale2, base2), a, c);
+            a = exp2_approx(a);
+            c = exp2_approx(c);
+            sums[q & 1] = f2_add(sums[q & 1], f2_make(a, c));
+            w[q] = pack_pair<BF16>(a, c);
           }
+          tmem_st_16(ts + b * kKeys, w);
+          tmem_st_16(ts + b * kKeys + 16, w + 16);
+          sum = f2_add(sums[0], sums[1]);
           float a, c;
-          f2_split(f2_add(sums[0], sums[1]), a, c);
+          f2_split(sum, a, c);
           l += a + c;
           tmem_st_wait();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->pfull[s]);
+        if (lane == 0) mbar_arrive(&sh->pfull[b]);
       }
       if (!ok) break;
       more = next_item(k + 1);
       if (more) load_q(item_at(k + 1));
 
       // ---- the item's end
-      const bool joined = !two && n > 1;  // two streams hold the same rows
       const bool whole = lo == 0 && it.hi == it.nt;
       const int slot = lo > 0 ? 0 : 1;
-      if (!whole) {
+      if (!whole && tid == 0) {
+        Meta* mt = p.meta + blockIdx.x;
         if (lo > 0)
-          meta_ends = it.hi == it.nt;
+          mt->head_ends = it.hi == it.nt;
         else
-          meta_tail = 1, meta_token = it.first + it.i0, meta_ntok = it.ntok, meta_head = it.h;
+          mt->tail = 1, mt->token = it.first + it.i0, mt->ntok = it.ntok, mt->head = it.h;
       }
-      if (ns == 0) {  // a single key tile: stream 0's alone
-        __syncwarp();
-        if (lane == 0) done(k);
-        continue;
-      }
-      ok = wait_warp(&sh->ofull[s], o_ph, p.err, abort);
+      ok = wait_warp(&sh->ofull, o_ph, p.err, abort);
       if (!ok) break;
       o_ph ^= 1;
-      if (joined && s == 1) {
-        sh->m1[row] = m;
-        sh->l1[row] = l;
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sh->ml1);
-          done(k);
-        }
-        b_ph ^= 1;
-        o1_pending = true;
-        continue;
-      }
-      float f0 = 1.f, f1 = 0.f;
-      if (joined) {
-        ok = wait_warp(&sh->ml1, b_ph, p.err, abort);  // stream 1 has seen O_1 complete
-        if (!ok) break;
-        const float m1 = sh->m1[row], l1 = sh->l1[row];
-        const float top = fmaxf(m, m1);
-        f0 = m == -INFINITY ? 0.f : exp2_approx(m - top);
-        f1 = m1 == -INFINITY ? 0.f : exp2_approx(m1 - top);
-        l = l * f0 + l1 * f1;
-        m = top;
-      }
+      if (n > 1) last_ph ^= 1;  // (completed before ofull)
       tc_fence_after();
       if (busy) {
         const bool bad = sh->bad[(k + 1) % kBadSlots] == k + 1;
         const float norm = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        f0 *= norm;
-        f1 *= norm;
         const size_t out_row = static_cast<size_t>(it.first + my_token) * p.Hq + it.h * p.G + (row - rt * p.G);
-        const int part_row = (two ? s * kTile : 0) + row;
         float* part = p.part + (static_cast<size_t>(blockIdx.x) * 2 + slot) * Sh::kPartFloats;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
           tmem_ld_32(to + c, o);
-          if (joined) {
-            float o1[32];
-            tmem_ld_32(to + D + c, o1);
-            tmem_ld_wait();
+          tmem_ld_wait();
 #pragma unroll
-            for (int q = 0; q < 32; ++q) o[q] = o[q] * f0 + o1[q] * f1;
-          } else {
-            tmem_ld_wait();
-#pragma unroll
-            for (int q = 0; q < 32; ++q) o[q] *= f0;
-          }
+          for (int q = 0; q < 32; ++q) o[q] *= norm;
           if (bad && live) {  // values that were kept out of the MMA
-            for (int key = max(full, lo * kTile); key < min(it.need, it.hi * kTile); ++key) {
+            for (int key = max(full, lo * kKeys); key < min(it.need, it.hi * kKeys); ++key) {
               if (!(visible(p, it, my_token, key) & 1)) continue;
               const int page = p.table[static_cast<long long>(it.b) * p.table_stride + (key >> p.page_shift)];
               if (page < 0 || page >= p.num_pages) continue;
@@ -935,33 +841,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                                   pack_pair<BF16>(o[8 * q + 4], o[8 * q + 5]),
                                   pack_pair<BF16>(o[8 * q + 6], o[8 * q + 7]));
           } else {
-            float4* dst = reinterpret_cast<float4*>(part + static_cast<size_t>(part_row) * D + c);
+            float4* dst = reinterpret_cast<float4*>(part + static_cast<size_t>(row) * D + c);
 #pragma unroll
             for (int q = 0; q < 8; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
           }
         }
         if (live) {
           if (!whole) {
-            part[kRowsMax * D + part_row] = m;
-            part[kRowsMax * D + kRowsMax + part_row] = l;
+            part[kTile * D + row] = m;
+            part[kTile * D + kTile + row] = l;
           } else if (p.lse) {
             p.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
         }
       }
-      if (joined) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->o1read);
-        b_ph ^= 1;
-      }
+      tc_fence_before();  // O has been read: the next P may be handed on
       __syncwarp();
       if (lane == 0) done(k);
-    }
-    if (tid == 0) {
-      Meta mt;
-      mt.tail = meta_tail, mt.head_ends = meta_ends, mt.token = meta_token, mt.ntok = meta_ntok, mt.head = meta_head;
-      p.meta[blockIdx.x] = mt;
     }
   }
 
@@ -973,9 +869,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     while (global_timer_ns() - t0 < 200000ull) {
     }
   }
-  if (warp == 10) {
+  if (warp == 6) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -991,7 +887,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Meta mt = p.meta[c];
   if (!mt.tail) return;
-  const int rows = mt.ntok * p.G, split = p.tok_tile * p.G;  // rows of the first tile
+  const int rows = mt.ntok * p.G;
   if (static_cast<int>(blockIdx.y) * kJoinRows >= rows) return;
   int last = c + 1;  // the CTA in which the item ends
   while (last < ctas - 1 && !p.meta[last].head_ends) ++last;
@@ -1000,9 +896,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
   };
   for (int r = blockIdx.y * kJoinRows + warp; r < min(rows, static_cast<int>(blockIdx.y + 1) * kJoinRows);
        r += kJoinThreads / 32) {
-    const int pr = r < split ? r : kTile + r - split;
     float top = -INFINITY;
-    for (int k = c + lane; k <= last; k += 32) top = fmaxf(top, partial(k)[kRowsMax * D + pr]);
+    for (int k = c + lane; k <= last; k += 32) top = fmaxf(top, partial(k)[kTile * D + r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float acc[kPer], sum = 0.f;
@@ -1011,14 +906,14 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
 #pragma unroll 4
     for (int k = c; k <= last; ++k) {
       const float* src = partial(k);
-      const float m = src[kRowsMax * D + pr];
+      const float m = src[kTile * D + r];
       const float w = m == -INFINITY ? 0.f : exp2_approx(m - top);
-      sum += w * src[kRowsMax * D + kRowsMax + pr];
+      sum += w * src[kTile * D + kTile + r];
       if constexpr (kPer == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<size_t>(pr) * D + lane * 4);
+        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<size_t>(r) * D + lane * 4);
         acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
       } else {
-        const float2 v = *reinterpret_cast<const float2*>(src + static_cast<size_t>(pr) * D + lane * 2);
+        const float2 v = *reinterpret_cast<const float2*>(src + static_cast<size_t>(r) * D + lane * 2);
         acc[0] += w * v.x, acc[1] += w * v.y;
       }
     }
@@ -1045,7 +940,7 @@ int make_cache_map(const void* base, const CacheStrides& cs, int D, int rows, in
                               static_cast<cuuint64_t>(Hkv), static_cast<cuuint64_t>(pages)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(cs.row) * 2, static_cast<cuuint64_t>(cs.head) * 2,
                                  static_cast<cuuint64_t>(cs.page) * 2};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kTile)), 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kKeys)), 1, 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1054,25 +949,26 @@ int make_cache_map(const void* base, const CacheStrides& cs, int D, int rows, in
              : NG_ERR_CUDA;
 }
 
-constexpr size_t kMetaBytes = 16384;
+constexpr size_t kMetaBytes = 32768;
 size_t attn_workspace_bytes(int D, const DeviceInfo& dev) {
   const size_t part = D == 128 ? Shape<128>::kPartFloats : Shape<64>::kPartFloats;
-  return kMetaBytes + static_cast<size_t>(dev.sm_count) * 2 * part * sizeof(float);
+  return kMetaBytes + static_cast<size_t>(dev.sm_count) * 4 * part * sizeof(float);
 }
 
 template <bool BF16, int D>
 int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnArgs& a, const DeviceInfo& dev,
                      cudaStream_t st) {
   constexpr int smem = Shape<D>::kSmem + static_cast<int>(sizeof(Shared<Shape<D>::kStages>));
-  static_assert(smem <= 227 * 1024, "ring and barriers must fit in shared memory");
+  static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs must fit in the shared memory of an SM");
+  const int ctas = 2 * dev.sm_count;
   auto kern = tree_attn_kernel<BF16, D>;
   static std::once_flag once[kMaxDevices];
   std::call_once(once[dev.device],
                  [&] { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-  if (int e = launch_chained(kern, dim3(dev.sm_count), dim3(kAttnThreads), smem, st, mk, mv, a)) return e;
-  const int rows = static_cast<int>(std::min<long long>(kRowsMax, static_cast<long long>(a.T) * a.G));
-  return launch_chained(tree_attn_join<BF16, D>, dim3(dev.sm_count, (rows + kJoinRows - 1) / kJoinRows),
-                        dim3(kJoinThreads), 0, st, a, dev.sm_count);
+  if (int e = launch_chained(kern, dim3(ctas), dim3(kAttnThreads), smem, st, mk, mv, a)) return e;
+  const int rows = static_cast<int>(std::min<long long>(kTile, static_cast<long long>(a.T) * a.G));
+  return launch_chained(tree_attn_join<BF16, D>, dim3(ctas, (rows + kJoinRows - 1) / kJoinRows),
+                        dim3(kJoinThreads), 0, st, a, ctas);
 }
 
 }  // namespace
