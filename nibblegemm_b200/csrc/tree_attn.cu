@@ -11,12 +11,11 @@
 //
 // Two persistent CTAs per SM, each warp-specialised:
 //   warps 0-3  softmax, one thread per row
-//   warp 4     TMA: the pages of a K or V tile into a ring of stages, one lane per
-//              page and 64-value half, 128-byte swizzle
+//   warp 4     walks this CTA's share of the work and hands out its items; TMA: the
+//              pages of a K or V tile into a ring of stages, one lane per page and
+//              64-value half, 128-byte swizzle
 //   warp 5     tcgen05.mma: S = Q K^T (128 x 64, both operands from shared
 //              memory), O += P V (P from tensor memory)
-//   warp 6     tensor-memory allocation; rows of V that no MMA may see (below)
-//   warp 7     walks this CTA's share of the work and hands out its items
 // Tensor memory: two buffers of scores (64 columns each; P is written over the
 // scores it comes from) and O (D columns).  While the softmax has one tile of scores
 // the tensor core computes the next one into the other buffer.  The two CTAs
@@ -52,9 +51,8 @@ namespace {
 
 constexpr int kTile = 128;         // rows of a query tile
 constexpr int kKeys = 64;          // keys of a key tile
-constexpr int kAttnThreads = 256;  // 8 warps, two CTAs an SM
+constexpr int kAttnThreads = 192;  // 6 warps; two CTAs an SM leave 168 registers a thread
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
-constexpr int kBadSlots = 8;
 constexpr int kItems = 4;          // work items handed out ahead
 constexpr int kMinUnits = 8;       // least work of a CTA, in key tiles
 constexpr int kItemUnits = 2;      // what an item costs beside its key tiles, in key tiles
@@ -199,7 +197,7 @@ struct Walk {
 
 template <int kStages>
 struct alignas(16) Shared {
-  uint64_t full[kStages], empty[kStages], vissued[kStages], vclean[kStages];
+  uint64_t full[kStages], empty[kStages];
   uint64_t sfull[2], pfull[2];  // by buffer
   uint64_t qfull, ofull, olast; // olast: all but the last P V of an item are done
   uint64_t item_full[kItems], item_empty[kItems];
@@ -208,7 +206,7 @@ struct alignas(16) Shared {
   Walk start;                   // where this CTA's share begins
   uint32_t tmem;
   int abort;
-  int bad[kBadSlots];
+  int bad[2];                   // by parity of the item: its number + 1 if it had V values that are not finite
 };
 
 // ---------------------------------------------------------------------------
@@ -377,8 +375,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
-      mbar_init(&sh->vissued[s], 1);
-      mbar_init(&sh->vclean[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh->sfull[b], 1);
@@ -389,16 +385,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     mbar_init(&sh->olast, 1);
     for (int s = 0; s < kItems; ++s) {
       mbar_init(&sh->item_full[s], 1);
-      mbar_init(&sh->item_empty[s], 7);  // TMA, MMA, V rows, 4 softmax warps
+      mbar_init(&sh->item_empty[s], 5);  // MMA, 4 softmax warps
     }
     sh->abort = 0;
     sh->start.u = sh->start.u1 = 0;  // no work, unless a thread finds some below
-    for (int i = 0; i < kBadSlots; ++i) sh->bad[i] = 0;
+    sh->bad[0] = sh->bad[1] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
-  if (warp == 6) tmem_alloc(&sh->tmem, 256);
+  if (warp == 5) tmem_alloc(&sh->tmem, 256);
   pdl_launch_next();
   pdl_wait_previous();
 
@@ -487,10 +483,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const int page_mask = (1 << p.page_shift) - 1;
     uint32_t st = 0, ph = 0;  // stage and parity of the next place
     bool ok = true;
-    for (int k = 0; ok && next_item(k); ++k) {
-      const Item it = item_at(k);
-      __syncwarp();
-      if (lane == 0) done(k);
+    Walk walk = sh->start;
+    for (int k = 0; ok; ++k) {
+      if (!wait_warp(&sh->item_empty[k % kItems], ((k / kItems) & 1) ^ 1, p.err, abort)) break;
+      Item it;  // (all lanes walk alike)
+      const bool more = walk.next(p, it);
+      if (!more) it.lo = it.hi = 0;
+      if (lane == 0) {
+        sh->items[k % kItems] = it;
+        mbar_arrive(&sh->item_full[k % kItems]);
+      }
+      if (!more) break;
       const int n = it.hi - it.lo;
       const int* row = p.table + static_cast<long long>(it.b) * p.table_stride;
       auto key_at = [&](int j) { return (it.lo + j) * kKeys + (piece << shift); };
@@ -500,12 +503,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         if (!wait_warp(&sh->empty[st], ph ^ 1, p.err, abort)) return false;
         const bool active = active_at(j);
         const unsigned votes = __ballot_sync(0xffffffffu, active);
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->full[st], __popc(votes) * piece_bytes);
-          // From here on the parity of full[st] means this use to the V-row warp, which
-          // only looks at some uses and could take another for it.
-          if (is_v && (it.lo + j + 1) * kKeys > it.full) mbar_arrive(&sh->vissued[st]);
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&sh->full[st], __popc(votes) * piece_bytes);
         __syncwarp();
         if (active) {
           if (page < 0 || page >= p.num_pages) {  // outside the pool: the load fills zeros
@@ -532,7 +530,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     constexpr uint32_t idesc_s = umma_idesc_f16(BF16, kTile, kKeys);
     constexpr uint32_t idesc_o = umma_idesc_f16(BF16, kTile, D) | (1u << 16);  // B (V) is N-major
     uint32_t st = 0, ph = 0;      // stage and parity of the next place
-    uint32_t clean_ph = 0;        // per stage: parity of its next cleaned use
     uint32_t q_ph = 0, p_ph = 0;  // parities of Q and of P (bit buffer)
     // broadcasts: known to be the same in all lanes
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
@@ -562,21 +559,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     bool ok = true;
     for (int k = 0; ok && next_item(k); ++k) {
       const Item& it = item_at(k);
-      const int lo = __shfl_sync(0xffffffffu, it.lo, 0), full = __shfl_sync(0xffffffffu, it.full, 0);
-      const int n = __shfl_sync(0xffffffffu, it.hi, 0) - lo;
+      const int n = __shfl_sync(0xffffffffu, it.hi, 0) - __shfl_sync(0xffffffffu, it.lo, 0);
       if (lane == 0) done(k);
-      const int clean0 = max(0, full / kKeys - lo);  // first tile with keys that not all rows see
       ok = wait_warp(&sh->qfull, q_ph, p.err, abort);
       q_ph ^= 1;
       ok = ok && scores(0) && (n == 1 || scores(1));
       for (int j = 0; ok && j < n; ++j) {  // O += P V of tile j, then the scores of tile j + 2
         const int b = j & 1;
-        ok = wait_warp(&sh->full[st], ph, p.err, abort);
-        if (ok && j >= clean0) {
-          ok = wait_warp(&sh->vclean[st], (clean_ph >> st) & 1, p.err, abort);
-          clean_ph ^= 1u << st;
-        }
-        ok = ok && wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort);
+        ok = wait_warp(&sh->full[st], ph, p.err, abort) && wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort);
         if (!ok) break;
         p_ph ^= 1u << b;
         tc_fence_after();
@@ -595,80 +585,55 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         if (j + 2 < n) ok = scores(b);
       }
     }
-  } else if (warp == 7) {
-    // ------------------------------------------------------------ the items
-    if (lane == 0) {
-      Walk walk = sh->start;
-      for (int k = 0;; ++k) {
-        if (!wait_bar(&sh->item_empty[k % kItems], ((k / kItems) & 1) ^ 1, p.err, abort)) break;
-        Item it;
-        const bool more = walk.next(p, it);
-        if (!more) it.lo = it.hi = 0;
-        sh->items[k % kItems] = it;
-        mbar_arrive(&sh->item_full[k % kItems]);
-        if (!more) break;
-      }
-    }
-  } else if (warp == 6) {
-    // ------------------------------------------------------------ V rows that no MMA may see
-    uint32_t place = 0, issued_ph = 0;
-    bool ok = true;
-    for (int k = 0; ok && next_item(k); ++k) {
-      const Item it = item_at(k);
-      __syncwarp();
-      if (lane == 0) done(k);
-      const int n = it.hi - it.lo, seq = k + 1;
-      for (int j = max(0, it.full / kKeys - it.lo); ok && j < n; ++j) {
-        const int key0 = (it.lo + j) * kKeys;
-        const uint32_t pl = place + min(n, j + 2) + j, st = pl % kStages;
-        ok = wait_warp(&sh->vissued[st], (issued_ph >> st) & 1, p.err, abort) &&
-             wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort);
-        if (!ok) break;
-        issued_ph ^= 1u << st;
-        unsigned char* tile = ring + st * Sh::kKvBytes;
-        bool bad = false;
-        for (int r = lane; r < kKeys; r += 32) {
-          const int key = key0 + r;
-          if (key < it.full) continue;
-          const bool beyond = key >= it.need;
-#pragma unroll
-          for (int hf = 0; hf < Sh::kHalves; ++hf) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(tile + hf * Sh::kKvHalf + r * 128 + (((c + lane) & 7) << 4));
-              if (beyond) {
-                *at = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 v = *at;
-              constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
-              auto infinite = [&](uint32_t w) { return ((w & kExp) + kOne) & 0x80008000u; };
-              if (infinite(v.x) | infinite(v.y) | infinite(v.z) | infinite(v.w)) {
-                auto clear = [&](uint32_t w) {
-                  const uint32_t f = infinite(w);
-                  return w & ~((f & 0x8000u ? 0xFFFFu : 0u) | (f & 0x80000000u ? 0xFFFF0000u : 0u));
-                };
-                *at = make_uint4(clear(v.x), clear(v.y), clear(v.z), clear(v.w));
-                bad = true;
-              }
-            }
-          }
-        }
-        if (bad) sh->bad[seq % kBadSlots] = seq;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->vclean[st]);
-      }
-      place += 2 * n;
-    }
   } else {
     // ------------------------------------------------------------ softmax, one thread per row
     const int row = tid & (kTile - 1);   // row of the tile
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t ts = tmem + lanes, to = tmem + 2 * kKeys + lanes;  // scores, O
     uint32_t s_ph = 0, o_ph = 0, last_ph = 0;  // parities: S (bit buffer), O, olast
+    uint32_t places = 0;                       // ring places of the items before
     bool ok = true;
     const int rt = row / p.G;
+
+    // What no MMA may see of the j-th V tile of an item of n: rows beyond the item's keys
+    // become zeros, and so do values that are not finite in rows that some query
+    // does not see (true if there are any).  Each softmax warp does 16 rows before it hands on
+    // its P, which the product with this tile waits for.  The use of the stage before this one
+    // is over: its place lies before that of K_j, whose scores are there; so the
+    // parity cannot stand for another use.
+    auto clean_values = [&](const Item& x, int k, int n, int j) {
+      const uint32_t pl = places + min(n, j + 2) + j, st = pl % kStages;
+      ok = wait_warp(&sh->full[st], (pl / kStages) & 1, p.err, abort);
+      if (!ok) return;
+      unsigned char* tile = ring + st * Sh::kKvBytes;
+      bool bad = false;
+      const int r = tid >> 1, key = (x.lo + j) * kKeys + r;  // two threads a row
+      if (key >= x.full) {
+        const bool beyond = key >= x.need;
+#pragma unroll
+        for (int q = 0; q < D / 16; ++q) {
+          const int c = q * 2 + (tid & 1);  // 16-byte chunk of the row
+          uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kKvHalf + r * 128 + (((c + r) & 7) << 4));
+          if (beyond) {
+            *at = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          const uint4 v = *at;
+          constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+          auto infinite = [&](uint32_t u) { return ((u & kExp) + kOne) & 0x80008000u; };
+          if (infinite(v.x) | infinite(v.y) | infinite(v.z) | infinite(v.w)) {
+            auto clear = [&](uint32_t u) {
+              const uint32_t f = infinite(u);
+              return u & ~((f & 0x8000u ? 0xFFFFu : 0u) | (f & 0x80000000u ? 0xFFFF0000u : 0u));
+            };
+            *at = make_uint4(clear(v.x), clear(v.y), clear(v.z), clear(v.w));
+            bad = true;
+          }
+        }
+      }
+      if (bad) sh->bad[k & 1] = k + 1;
+      fence_proxy_async_smem();
+    };
 
     // The item's Q rows into shared memory (128-byte swizzle).
     auto load_q = [&](const Item& x) {
@@ -782,11 +747,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           l += a + c;
           tmem_st_wait();
         }
+        if ((lo + j + 1) * kKeys > full) {
+          clean_values(it, k, n, j);
+          if (!ok) break;
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->pfull[b]);
       }
       if (!ok) break;
+      places += 2 * n;
       more = next_item(k + 1);
       if (more) load_q(item_at(k + 1));
 
@@ -806,7 +776,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (n > 1) last_ph ^= 1;  // (completed before ofull)
       tc_fence_after();
       if (busy) {
-        const bool bad = sh->bad[(k + 1) % kBadSlots] == k + 1;
+        const bool bad = sh->bad[k & 1] == k + 1;
         const float norm = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const size_t out_row = static_cast<size_t>(it.first + my_token) * p.Hq + it.h * p.G + (row - rt * p.G);
         float* part = p.part + (static_cast<size_t>(blockIdx.x) * 2 + slot) * Sh::kPartFloats;
@@ -869,7 +839,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     while (global_timer_ns() - t0 < 200000ull) {
     }
   }
-  if (warp == 6) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
@@ -877,7 +847,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 
 // Joins the partials of the items that lie in several CTAs, in CTA order.  Block
 // (c, y): the item that begins in CTA c and goes on, rows y * kJoinRows on.
-constexpr int kJoinRows = 16, kJoinThreads = 128;
+constexpr int kJoinRows = 8, kJoinThreads = 256;
 
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArgs p, int ctas) {
@@ -903,7 +873,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
     float acc[kPer], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int k = c; k <= last; ++k) {
       const float* src = partial(k);
       const float m = src[kTile * D + r];
