@@ -54,8 +54,8 @@ constexpr int kKeys = 64;          // keys of a key tile
 constexpr int kAttnThreads = 192;  // 6 warps; two CTAs an SM leave 168 registers a thread
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
 constexpr int kItems = 4;          // work items handed out ahead
-constexpr int kMinUnits = 8;       // least work of a CTA, in key tiles
-constexpr int kItemUnits = 2;      // what an item costs beside its key tiles, in key tiles
+constexpr int kMinUnits = 4;       // least work of a CTA, in key tiles
+constexpr int kItemUnits = 4;      // what an item costs beside its key tiles, in key tiles
 
 // A work item as one CTA sees it.
 struct alignas(16) Item {
@@ -592,6 +592,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const uint32_t ts = tmem + lanes, to = tmem + 2 * kKeys + lanes;  // scores, O
     uint32_t s_ph = 0, o_ph = 0, last_ph = 0;  // parities: S (bit buffer), O, olast
     uint32_t places = 0;                       // ring places of the items before
+    int filled = kTile;                        // rows of Q in shared memory that may not be zero
     bool ok = true;
     const int rt = row / p.G;
 
@@ -635,7 +636,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       fence_proxy_async_smem();
     };
 
-    // The item's Q rows into shared memory (128-byte swizzle).
+    // The item's Q rows into shared memory (128-byte swizzle), zeros in the rows beyond:
+    // products with zero take a fraction of the power, and under the power limit
+    // of a long decode that is clock rate (64 x 8192 single tokens of 4 rows: 242 -> 224 us).
     auto load_q = [&](const Item& x) {
       const int rows = x.ntok * p.G;
       constexpr int kChunks = D / 8, kStep = kTile / kChunks;  // a thread: one chunk of every kStep-th row
@@ -643,17 +646,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const uint16_t* src = p.q + static_cast<long long>(x.first + x.i0) * p.q_token +
                             static_cast<long long>(x.h) * p.G * p.q_head + c * 8;
       unsigned char* dst = smem + (c >> 3) * Sh::kQHalf;
-      for (int rr = r0; rr < rows; rr += 8 * kStep) {  // eight loads in flight
+      const int fill = max(rows, filled);  // rows that must be written: the item's, the ones in use before
+      filled = rows;
+      for (int rr = r0; rr < fill; rr += 8 * kStep) {  // eight loads in flight
         uint4 v[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           const int r = rr + q * kStep, tk = r / p.G;
+          v[q] = make_uint4(0, 0, 0, 0);
           if (r < rows) v[q] = ld_ro_v4(src + tk * p.q_token + (r - tk * p.G) * p.q_head);
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           const int r = rr + q * kStep;
-          if (r < rows) *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[q];
+          if (r < fill) *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[q];
         }
       }
       fence_proxy_async_smem();
@@ -727,7 +733,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
               tmem_st_16(to + c, o);
             }
           }
-          const float base = m == -INFINITY ? 0.f : -m;
+          const float base = !live ? -INFINITY : m == -INFINITY ? 0.f : -m;  // (no row: P = 0)
           const f2 base2 = f2_make(base, base);
           f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
