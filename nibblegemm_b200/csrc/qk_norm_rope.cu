@@ -10,9 +10,15 @@
 // is off by 6e-3 rad at position 100,000.
 //
 // A row of D values is held by D / 8 lanes, 16 bytes each, so a warp works on
-// 256 / D rows at a time; the sum of squares is a shuffle reduction within the
-// row and the rotation partner is a shuffle across half of the rotated lanes.  A
-// warp keeps one token, so its cosines and sines are computed once for its rows.
+// 256 / D rows at a time.  Weight and rotation are folded into two factors per value,
+//   out_i = inv (x_i (w_i c_i) + x_p (w_p s_i)),  p the partner of i, s_i signed,
+// which a warp works out once for its token and section (q or k); the partner comes
+// by a shuffle of the raw 16-bit values (four words for eight of them).  The sum of squares is a
+// shuffle reduction within the row.  Each half of a rotated pair of lanes evaluates
+// half of their common sines.  v rows are copied without being looked at.
+//
+// Bound: HBM for many tokens.  Four rows are loaded ahead (with one, the loads
+// of a warp were exposed one after another).
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -43,84 +49,159 @@ struct NormRopeArgs {
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const NormRopeArgs p) {
   constexpr int kLanes = D / 8;        // lanes per row
-  constexpr int kRows = 32 / kLanes;   // rows per warp and iteration
+  constexpr int kRows = 32 / kLanes;   // rows per warp and step
+  constexpr int kAhead = 4;            // steps whose rows are loaded together
   pdl_launch_next();
   pdl_wait_previous();
   const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
   const int gw = blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);
   const int m = gw / p.chunks, chunk = gw % p.chunks;
   if (m >= p.M) return;
-  const int rows = p.Hq + 2 * p.Hkv;
-  const int steps = (rows + kRows - 1) / kRows;
+  // Steps of the three sections, and this warp's run of them.
+  const int q_steps = (p.Hq + kRows - 1) / kRows, k_steps = (p.Hkv + kRows - 1) / kRows;
+  const int steps = q_steps + 2 * k_steps;
   const int s0 = steps * chunk / p.chunks, s1 = steps * (chunk + 1) / p.chunks;
+
+  const uint16_t* src = p.qkv + static_cast<size_t>(m) * p.qkv_stride + l * 8;
+  const int slot = p.slots[m];
+  const bool stored = slot >= 0 && slot < p.num_rows;
+  if (slot >= p.num_rows && lane == 0) atomicOr(p.err, kErrBadIndex);
+  const size_t cache_row = stored ? static_cast<size_t>(slot >> p.page_shift) * p.cs.page +
+                                        static_cast<size_t>(slot & ((1 << p.page_shift) - 1)) * p.cs.row + l * 8
+                                  : 0;
+
+  // The rows of up to kAhead steps from step s on, all of one section.
+  auto end_of = [&](int section) { return section == 0 ? min(s1, q_steps) : section == 1 ? min(s1, q_steps + k_steps) : s1; };
+  auto section_of = [&](int s) { return s < q_steps ? 0 : s < q_steps + k_steps ? 1 : 2; };
+  auto row_of = [&](int section, int s) { return (s - (section ? q_steps + (section - 1) * k_steps : 0)) * kRows + sub; };
+  auto load = [&](int s, uint4 (&x)[kAhead]) {
+    const int section = section_of(s), heads = section ? p.Hkv : p.Hq, end = end_of(section);
+    const uint16_t* rows = src + static_cast<size_t>(section ? p.Hq + (section - 1) * p.Hkv : 0) * D;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = row_of(section, s + i);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (s + i < end && r < heads) x[i] = ld_ro_v4(rows + static_cast<size_t>(r) * D);
+    }
+  };
+  uint4 x[kAhead];
+  load(s0, x);  // before the sines: they wait for the position, and these need not
 
   const int half8 = p.rot / 16;  // lanes of the rotated first half
   const bool rotated = l < 2 * half8, low = l < half8;
-  const int partner = rotated ? (low ? lane + half8 : lane - half8) : lane;
-  float cs[8], sn[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
-  if (rotated) {
-    const unsigned long long pos = static_cast<unsigned long long>(static_cast<long long>(p.positions[m]));
-    const long long* t = p.turns + (low ? l : l - half8) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int phase = static_cast<int>(static_cast<unsigned long long>(t[j]) * pos >> 32);
-      sincospif(static_cast<float>(phase) * 4.656612873077393e-10f, &sn[j], &cs[j]);  // 2^-31 half turns
-      if (low) sn[j] = -sn[j];
-    }
-  }
-  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+  const int other = low ? l + half8 : l - half8;  // the partner's place in the row
+  const int partner = rotated ? lane - l + other : lane;
+  const unsigned pairs = __ballot_sync(0xffffffffu, rotated);  // whole pairs of lanes
   const bool normed = p.q_weight != nullptr;
-  if (normed) {
-    wq = ld_ro_v4(p.q_weight + l * 8);
-    wk = ld_ro_v4(p.k_weight + l * 8);
+  float cs[8], sn[8];
+  if (s0 < q_steps + k_steps) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
+    if (rotated) {
+      // A pair of lanes has the same eight frequencies: the low lane evaluates the
+      // first four, the high one the others.
+      const unsigned long long pos = static_cast<unsigned long long>(static_cast<long long>(p.positions[m]));
+      const long long* t = p.turns + (low ? l * 8 : other * 8 + 4);
+      float c4[4], n4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int phase = static_cast<int>(static_cast<unsigned long long>(t[j]) * pos >> 32);
+        sincospif(static_cast<float>(phase) * 4.656612873077393e-10f, &n4[j], &c4[j]);  // 2^-31 half turns
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float co = __shfl_sync(pairs, c4[j], partner), no = __shfl_sync(pairs, n4[j], partner);
+        cs[j] = low ? c4[j] : co;
+        cs[4 + j] = low ? co : c4[j];
+        sn[j] = low ? -n4[j] : no;
+        sn[4 + j] = low ? -no : n4[j];
+      }
+    }
   }
-  const int slot = p.slots[m];
-  const bool stored = slot >= 0 && slot < p.num_rows;
-  if (slot >= p.num_rows && l == 0) atomicOr(p.err, kErrBadIndex);
-  const size_t cache_row = stored ? static_cast<size_t>(slot >> p.page_shift) * p.cs.page +
-                                        static_cast<size_t>(slot & ((1 << p.page_shift) - 1)) * p.cs.row
-                                  : 0;
-  const uint16_t* src = p.qkv + static_cast<size_t>(m) * p.qkv_stride;
-  for (int s = s0; s < s1; ++s) {
-    const int r = s * kRows + sub;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < rows) x = ld_ro_v4(src + static_cast<size_t>(r) * D + l * 8);
-    float f[8];
-    unpack8<BF16>(x, f);
-    if (normed) {
-      float ss = 0.f;
+
+  f2 fc[4], fs[4];
+  int have = -1;  // section whose factors fc and fs are
+  for (int s = s0; s < s1;) {
+    const int section = section_of(s);
+    const int next = min(s + kAhead, end_of(section));
+    uint4 ahead[kAhead];
+    if (next < s1) load(next, ahead);
+    if (section == 2) {  // v rows, as they are
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+      for (int i = 0; i < kAhead; ++i) {
+        const int r = row_of(2, s + i);
+        if (s + i < next && r < p.Hkv && stored)
+          *reinterpret_cast<uint4*>(p.v_cache + cache_row + r * p.cs.head) = x[i];
+      }
+    } else if (section == 0 || stored) {
+      if (section != have) {
+        have = section;
+        float wo[8], wp[8];
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-      float w[8];
-      unpack8<BF16>(r < p.Hq ? wq : wk, w);
+        for (int j = 0; j < 8; ++j) wo[j] = wp[j] = 1.f;
+        if (normed) {
+          const uint16_t* w = section ? p.k_weight : p.q_weight;
+          unpack8<BF16>(ld_ro_v4(w + l * 8), wo);
+          unpack8<BF16>(ld_ro_v4(w + (rotated ? other : l) * 8), wp);
+        }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = f[j] * inv * w[j];
+        for (int j = 0; j < 4; ++j) {
+          fc[j] = f2_make(wo[2 * j] * cs[2 * j], wo[2 * j + 1] * cs[2 * j + 1]);
+          fs[j] = f2_make(wp[2 * j] * sn[2 * j], wp[2 * j + 1] * sn[2 * j + 1]);
+        }
+      }
+      const int heads = section ? p.Hkv : p.Hq;
+      uint16_t* dst = section ? p.k_cache + cache_row : p.q_out + static_cast<size_t>(m) * p.Hq * D + l * 8;
+      const long long dst_head = section ? p.cs.head : D;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (s + i >= next) break;
+        const int r = row_of(section, s + i);
+        uint4 y;
+        y.x = __shfl_sync(0xffffffffu, x[i].x, partner);
+        y.y = __shfl_sync(0xffffffffu, x[i].y, partner);
+        y.z = __shfl_sync(0xffffffffu, x[i].z, partner);
+        y.w = __shfl_sync(0xffffffffu, x[i].w, partner);
+        if (!rotated) y = make_uint4(0, 0, 0, 0);  // (0 * inf would not be 0)
+        float f[8], g[8];
+        unpack8<BF16>(x[i], f);
+        unpack8<BF16>(y, g);
+        float inv = 1.f;
+        if (normed) {
+          f2 sq = f2_make(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f2 v = f2_make(f[2 * j], f[2 * j + 1]);
+            sq = f2_fma(v, v, sq);
+          }
+          float lo, hi;
+          f2_split(sq, lo, hi);
+          float ss = lo + hi;
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          inv = rsqrtf(ss * (1.f / D) + p.eps);
+        }
+        const f2 inv2 = f2_make(inv, inv);
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f2 t = f2_fma(f2_make(f[2 * j], f[2 * j + 1]), fc[j],
+                              f2_mul(f2_make(g[2 * j], g[2 * j + 1]), fs[j]));
+          f2_split(f2_mul(t, inv2), o[2 * j], o[2 * j + 1]);
+        }
+        if (r < heads) *reinterpret_cast<uint4*>(dst + r * dst_head) = pack8<BF16>(o);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float other = __shfl_sync(0xffffffffu, f[j], partner);
-      f[j] = f[j] * cs[j] + (rotated ? other * sn[j] : 0.f);
-    }
-    if (r < p.Hq) {
-      *reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(m) * p.Hq + r) * D + l * 8) = pack8<BF16>(f);
-    } else if (r < rows && stored) {
-      if (r < p.Hq + p.Hkv)
-        *reinterpret_cast<uint4*>(p.k_cache + cache_row + (r - p.Hq) * p.cs.head + l * 8) = pack8<BF16>(f);
-      else
-        *reinterpret_cast<uint4*>(p.v_cache + cache_row + (r - p.Hq - p.Hkv) * p.cs.head + l * 8) = x;
-    }
+    for (int i = 0; i < kAhead; ++i) x[i] = ahead[i];
+    s = next;
   }
 }
 
 template <bool BF16, int D>
 int launch_norm_rope(NormRopeArgs a, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int kRows = 256 / D;
-  const int steps = (a.Hq + 2 * a.Hkv + kRows - 1) / kRows;
+  const int steps = (a.Hq + kRows - 1) / kRows + 2 * ((a.Hkv + kRows - 1) / kRows);
   // Few tokens: one step a warp, to spread the rows over the SMs.  Many: one
   // warp a token, so the sines are computed once.
   const long long want = static_cast<long long>(dev.sm_count) * 32;
