@@ -164,6 +164,32 @@ int64_t check_table(const torch::Tensor& t, const torch::Device& dev, int64_t B)
   return B > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1));
 }
 
+// Several small outputs out of one allocation: each begins on a 16-byte boundary of
+// `buffer` (uint8).  Made without the dispatcher, which takes most of a microsecond
+// for each empty() or view.
+class Slices {
+ public:
+  Slices(int64_t bytes, const torch::Device& dev)
+      : buffer_(torch::empty({bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev))) {}
+  static int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+  torch::Tensor take(torch::IntArrayRef sizes, torch::ScalarType type) {
+    int64_t n = 1;
+    for (const auto s : sizes) n *= s;
+    const int64_t item = static_cast<int64_t>(c10::elementSize(type));
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer_.storage()), buffer_.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(used_ / item);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    used_ += padded(n * item);
+    TORCH_INTERNAL_ASSERT(used_ <= buffer_.numel());
+    return t;
+  }
+
+ private:
+  torch::Tensor buffer_;
+  int64_t used_ = 0;
+};
+
 std::tuple<std::vector<std::optional<torch::Tensor>>, int64_t> paged_plan(
     torch::Tensor cached, torch::Tensor fresh, torch::Tensor held, torch::Tensor table, torch::Tensor free_pages,
     int64_t page_size, int64_t num_tokens, std::optional<torch::Tensor> parents, int64_t mask_words,
@@ -188,11 +214,15 @@ std::tuple<std::vector<std::optional<torch::Tensor>>, int64_t> paged_plan(
     TORCH_CHECK(cursor->size(0) == 1, "cursor must have one entry");
   }
   const c10::cuda::CUDAGuard guard(dev);
-  auto cu = torch::empty({B + 1}, cached.options()), slots = torch::empty({num_tokens}, cached.options()),
-       positions = torch::empty({num_tokens}, cached.options()), kv = torch::empty({B}, cached.options()),
-       held_out = torch::empty({B}, cached.options()), taken = torch::empty({1}, cached.options());
+  TORCH_CHECK(mask_words >= 0 && mask_words <= 64, "mask_words must be 0..64");
+  const int64_t token = Slices::padded(num_tokens * 4), request = Slices::padded(B * 4);
+  Slices slices(Slices::padded((B + 1) * 4) + 2 * token + 2 * request + 16 + Slices::padded(num_tokens * mask_words * 8),
+                dev);
+  auto cu = slices.take({B + 1}, torch::kInt), slots = slices.take({num_tokens}, torch::kInt),
+       positions = slices.take({num_tokens}, torch::kInt), kv = slices.take({B}, torch::kInt),
+       held_out = slices.take({B}, torch::kInt), taken = slices.take({1}, torch::kInt);
   std::optional<torch::Tensor> mask;
-  if (mask_words > 0) mask = torch::empty({num_tokens, mask_words}, cached.options().dtype(torch::kLong));
+  if (mask_words > 0) mask = slices.take({num_tokens, mask_words}, torch::kLong);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   const int st = ng_paged_plan(
       cached.data_ptr<int>(), fresh.data_ptr<int>(), held.data_ptr<int>(), table.data_ptr<int>(), stride,
@@ -303,8 +333,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, int64_t> 
   TORCH_CHECK(max_path >= 1 && max_path <= 512, "max_path must be 1..512");
   const int64_t stride = check_table(table, dev, B);
   const c10::cuda::CUDAGuard guard(dev);
-  auto accepted = torch::empty({B}, kv_lens.options()), path = torch::empty({B, max_path}, kv_lens.options()),
-       bonus = torch::empty({B}, draft.options()), kv_out = torch::empty({B}, kv_lens.options());
+  Slices slices(2 * Slices::padded(B * 4) + Slices::padded(B * max_path * 4) + Slices::padded(B * 8), dev);
+  auto accepted = slices.take({B}, torch::kInt), path = slices.take({B, max_path}, torch::kInt),
+       bonus = slices.take({B}, torch::kLong), kv_out = slices.take({B}, torch::kInt);
   if (B == 0) return {accepted, path, bonus, kv_out, 0};
   if (T == 0) {
     accepted.zero_();

@@ -5,13 +5,16 @@
 // Then, for every layer, cache row (before + i) <- row (before + path_i), with
 // before = kv - n the rows in front of the tree: the kept nodes become the
 // context's last rows and the rest is free to be written over.  path is
-// increasing, so row i is never the source of a later move once written
-// (path_j > path_i >= i for j > i): copying in the order of i needs no buffer.
+// increasing and path_i >= i, so a row that a move has written is never the source of a later
+// move (path_j >= j > i): the rows of a few moves can be read together, and
+// no buffer is needed.
 //
-// One CTA per (request, layer, share of the heads); every CTA repeats the walk (a
-// few steps over the tree's nodes, one warp, children found by ballot) rather
-// than wait for another kernel.  A thread owns 16-byte columns of a row and
-// moves them path step by path step, so moves of one column stay in order.
+// One CTA per (request, a few layers, share of the heads); every CTA repeats the walk
+// rather than wait for another kernel.  The walk is bound by latency, so all nodes
+// look up at once whether they follow their parent, each parent keeps its first such child
+// (an atomic minimum, whose order does not matter), and the path is a chase through shared
+// memory: two rounds of global loads instead of two for every node of the path.
+// Trees of more nodes than fit there are walked with a ballot over the children.
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -21,6 +24,7 @@ namespace {
 
 constexpr int kCommitThreads = 128;
 constexpr int kCommitMaxPath = 512;
+constexpr int kCommitNodes = 2048;  // nodes of a tree whose children are found in shared memory
 
 struct CommitArgs {
   const long long* draft;
@@ -34,7 +38,7 @@ struct CommitArgs {
   uint4* k_cache;
   uint4* v_cache;
   long long s_layer, s_page, s_row, s_head;  // in 16-byte units
-  int B, T, Hkv, vecs, num_pages, page_shift, max_path;
+  int B, T, layers, Hkv, vecs, num_pages, page_shift, max_path;
   int* accepted;
   int* path;
   long long* bonus;
@@ -44,37 +48,53 @@ struct CommitArgs {
 
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs p) {
   __shared__ int path[kCommitMaxPath];
+  __shared__ int child[kCommitNodes];
+  __shared__ long long from[kCommitMaxPath], to[kCommitMaxPath];  // 16-byte units in a layer, -1: not mapped
   __shared__ int count_s;
   pdl_launch_next();
   pdl_wait_previous();
-  const int b = blockIdx.x, layer = blockIdx.y;
+  const int b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31;
   const int first = min(max(p.cu[b], 0), p.T), end = min(max(p.cu[b + 1], first), p.T);
   const int n = end - first;
   const int kv = p.kv[b];
+  const bool any = n > 0 && kv >= n;
+  if (any && n <= kCommitNodes) {
+    for (int c = tid; c < n; c += kCommitThreads) child[c] = n;
+    __syncthreads();
+    for (int c = tid; c < n; c += kCommitThreads) {
+      const int up = p.parents[first + c];
+      if (up >= 0 && up < c && p.draft[first + c] == p.next[first + up]) atomicMin(&child[up], c);
+    }
+    __syncthreads();
+  }
   if (tid < 32) {
     int count = 0;
-    if (n > 0 && kv >= n) {
+    if (any) {
       int cur = 0;
       for (;;) {
         if (lane == 0) path[count] = cur;
         ++count;
         if (count >= p.max_path) break;
-        const long long want = p.next[first + cur];
-        int found = -1;
-        for (int c0 = cur + 1; c0 < n && found < 0; c0 += 32) {  // children come after their parent
-          const int c = c0 + lane;
-          const bool hit = c < n && p.parents[first + c] == cur && p.draft[first + c] == want;
-          const unsigned vote = __ballot_sync(0xffffffffu, hit);
-          if (vote) found = c0 + __ffs(vote) - 1;
+        int found = n;
+        if (n <= kCommitNodes) {
+          found = child[cur];
+        } else {
+          const long long want = p.next[first + cur];
+          for (int c0 = cur + 1; c0 < n && found == n; c0 += 32) {  // children come after their parent
+            const int c = c0 + lane;
+            const bool hit = c < n && p.parents[first + c] == cur && p.draft[first + c] == want;
+            const unsigned vote = __ballot_sync(0xffffffffu, hit);
+            if (vote) found = c0 + __ffs(vote) - 1;
+          }
         }
-        if (found < 0) break;
+        if (found == n) break;
         cur = found;
       }
     }
     __syncwarp();
     if (lane == 0) count_s = count;
-    if (layer == 0 && blockIdx.z == 0) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) {
       if (lane == 0) {
         p.accepted[b] = count;
         p.bonus[b] = count ? p.next[first + path[count - 1]] : -1;
@@ -87,27 +107,46 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   }
   __syncthreads();
   const int count = count_s, before = kv - n;
-  const int ps_mask = (1 << p.page_shift) - 1;
   const int* row = p.table + static_cast<size_t>(b) * p.table_stride;
-  auto offset = [&](int at) -> long long {  // 16-byte units of cache row `at`, or -1
+  auto offset = [&](int at) -> long long {  // of cache row `at`
     const int blk = at >> p.page_shift;
     const int page = blk < p.table_width ? row[blk] : -1;
     if (page < 0 || page >= p.num_pages) return -1;
-    return page * p.s_page + (at & ps_mask) * p.s_row;
+    return page * p.s_page + (at & ((1 << p.page_shift) - 1)) * p.s_row;
   };
-  const int columns = p.Hkv * p.vecs;
-  const size_t base = static_cast<size_t>(layer) * p.s_layer;
-  for (int col = blockIdx.z * kCommitThreads + tid; col < columns; col += gridDim.z * kCommitThreads) {
-    const size_t at = base + static_cast<size_t>(col / p.vecs) * p.s_head + col % p.vecs;
-    for (int i = 0; i < count; ++i) {
-      if (path[i] == i) continue;
-      const long long from = offset(before + path[i]), to = offset(before + i);
-      if (from < 0 || to < 0) {
+  for (int i = tid; i < count; i += kCommitThreads) {
+    from[i] = to[i] = -1;
+    if (path[i] != i) {
+      from[i] = offset(before + path[i]);
+      to[i] = offset(before + i);
+      if (from[i] < 0 || to[i] < 0) {
         atomicOr(p.err, kErrBadIndex);
-        continue;
+        from[i] = -1;
       }
-      p.k_cache[at + to] = p.k_cache[at + from];
-      p.v_cache[at + to] = p.v_cache[at + from];
+    }
+  }
+  __syncthreads();
+  constexpr int kBatch = 4;  // moves whose rows are read together
+  const int columns = p.Hkv * p.vecs;
+  for (int layer = blockIdx.y; layer < p.layers; layer += gridDim.y) {
+    for (int col = blockIdx.z * kCommitThreads + tid; col < columns; col += gridDim.z * kCommitThreads) {
+      const size_t at = static_cast<size_t>(layer) * p.s_layer + static_cast<size_t>(col / p.vecs) * p.s_head +
+                        col % p.vecs;
+      for (int i0 = 0; i0 < count; i0 += kBatch) {
+        uint4 k[kBatch], v[kBatch];
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q)
+          if (i0 + q < count && from[i0 + q] >= 0) {
+            k[q] = p.k_cache[at + from[i0 + q]];
+            v[q] = p.v_cache[at + from[i0 + q]];
+          }
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q)
+          if (i0 + q < count && from[i0 + q] >= 0) {
+            p.k_cache[at + to[i0 + q]] = k[q];
+            p.v_cache[at + to[i0 + q]] = v[q];
+          }
+      }
     }
   }
 }
@@ -138,9 +177,13 @@ extern "C" int ng_tree_commit(const long long* draft, const int* parents, const 
   if (int st = current_device_info(&dev)) return st;
   const CommitArgs a{draft, parents, next, cu_new, kv_lens, block_table, table_stride, table_width,
                      static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), stride_layer / 8,
-                     stride_page / 8, stride_row / 8, stride_head / 8, B, T, Hkv, D / 8, num_pages,
+                     stride_page / 8, stride_row / 8, stride_head / 8, B, T, layers, Hkv, D / 8, num_pages,
                      log2_of(page_size), max_path, accepted, path, bonus, kv_out, dev.err};
-  const int shares = std::max(1, (Hkv * (D / 8) + kCommitThreads - 1) / kCommitThreads);
-  return launch_chained(tree_commit_kernel, dim3(B, layers, std::min(shares, 64)), dim3(kCommitThreads), 0,
+  const int shares = std::min(64, std::max(1, (Hkv * (D / 8) + kCommitThreads - 1) / kCommitThreads));
+  // A CTA takes several layers once every SM has eight CTAs: the walk is then
+  // repeated less often (64 requests x 32 layers: NNN us with one layer a CTA, MMM us so).
+  const long long ctas = static_cast<long long>(B) * layers * shares;
+  const int per = static_cast<int>(std::min<long long>(layers, std::max<long long>(1, ctas / (8 * dev.sm_count))));
+  return launch_chained(tree_commit_kernel, dim3(B, (layers + per - 1) / per, shares), dim3(kCommitThreads), 0,
                         static_cast<cudaStream_t>(stream), a);
 }
