@@ -9,8 +9,9 @@
 // move (path_j >= j > i): the rows of a few moves can be read together, and
 // no buffer is needed.
 //
-// One CTA per (request, a few layers, share of the heads); every CTA repeats the walk
-// rather than wait for another kernel.  The walk is bound by latency, so all nodes
+// One CTA per (request, layer, share of the heads); every CTA repeats the walk
+// rather than wait for another kernel (several layers a CTA, to walk less often,
+// measured no faster).  The walk is bound by latency, so all nodes
 // look up at once whether they follow their parent, each parent keeps its first such child
 // (an atomic minimum, whose order does not matter), and the path is a chase through shared
 // memory: two rounds of global loads instead of two for every node of the path.
@@ -38,7 +39,7 @@ struct CommitArgs {
   uint4* k_cache;
   uint4* v_cache;
   long long s_layer, s_page, s_row, s_head;  // in 16-byte units
-  int B, T, layers, Hkv, vecs, num_pages, page_shift, max_path;
+  int B, T, Hkv, vecs, num_pages, page_shift, max_path;
   int* accepted;
   int* path;
   long long* bonus;
@@ -128,25 +129,23 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   __syncthreads();
   constexpr int kBatch = 4;  // moves whose rows are read together
   const int columns = p.Hkv * p.vecs;
-  for (int layer = blockIdx.y; layer < p.layers; layer += gridDim.y) {
-    for (int col = blockIdx.z * kCommitThreads + tid; col < columns; col += gridDim.z * kCommitThreads) {
-      const size_t at = static_cast<size_t>(layer) * p.s_layer + static_cast<size_t>(col / p.vecs) * p.s_head +
-                        col % p.vecs;
-      for (int i0 = 0; i0 < count; i0 += kBatch) {
-        uint4 k[kBatch], v[kBatch];
+  for (int col = blockIdx.z * kCommitThreads + tid; col < columns; col += gridDim.z * kCommitThreads) {
+    const size_t at = static_cast<size_t>(blockIdx.y) * p.s_layer + static_cast<size_t>(col / p.vecs) * p.s_head +
+                      col % p.vecs;
+    for (int i0 = 0; i0 < count; i0 += kBatch) {
+      uint4 k[kBatch], v[kBatch];
 #pragma unroll
-        for (int q = 0; q < kBatch; ++q)
-          if (i0 + q < count && from[i0 + q] >= 0) {
-            k[q] = p.k_cache[at + from[i0 + q]];
-            v[q] = p.v_cache[at + from[i0 + q]];
-          }
+      for (int q = 0; q < kBatch; ++q)
+        if (i0 + q < count && from[i0 + q] >= 0) {
+          k[q] = p.k_cache[at + from[i0 + q]];
+          v[q] = p.v_cache[at + from[i0 + q]];
+        }
 #pragma unroll
-        for (int q = 0; q < kBatch; ++q)
-          if (i0 + q < count && from[i0 + q] >= 0) {
-            p.k_cache[at + to[i0 + q]] = k[q];
-            p.v_cache[at + to[i0 + q]] = v[q];
-          }
-      }
+      for (int q = 0; q < kBatch; ++q)
+        if (i0 + q < count && from[i0 + q] >= 0) {
+          p.k_cache[at + to[i0 + q]] = k[q];
+          p.v_cache[at + to[i0 + q]] = v[q];
+        }
     }
   }
 }
@@ -177,13 +176,9 @@ extern "C" int ng_tree_commit(const long long* draft, const int* parents, const 
   if (int st = current_device_info(&dev)) return st;
   const CommitArgs a{draft, parents, next, cu_new, kv_lens, block_table, table_stride, table_width,
                      static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), stride_layer / 8,
-                     stride_page / 8, stride_row / 8, stride_head / 8, B, T, layers, Hkv, D / 8, num_pages,
+                     stride_page / 8, stride_row / 8, stride_head / 8, B, T, Hkv, D / 8, num_pages,
                      log2_of(page_size), max_path, accepted, path, bonus, kv_out, dev.err};
   const int shares = std::min(64, std::max(1, (Hkv * (D / 8) + kCommitThreads - 1) / kCommitThreads));
-  // A CTA takes several layers once every SM has eight CTAs: the walk is then
-  // repeated less often (64 requests x 32 layers: NNN us with one layer a CTA, MMM us so).
-  const long long ctas = static_cast<long long>(B) * layers * shares;
-  const int per = static_cast<int>(std::min<long long>(layers, std::max<long long>(1, ctas / (8 * dev.sm_count))));
-  return launch_chained(tree_commit_kernel, dim3(B, (layers + per - 1) / per, shares), dim3(kCommitThreads), 0,
+  return launch_chained(tree_commit_kernel, dim3(B, layers, shares), dim3(kCommitThreads), 0,
                         static_cast<cudaStream_t>(stream), a);
 }
