@@ -11,6 +11,7 @@ from .decode_model import LLAMA3_8B_MODEL, LLAMA3_70B_MODEL, Llama3Decoder
 from .importers import from_autogptq, to_autogptq
 from .paged import (PagedPlan, TreeCommit, paged_cache, paged_plan, qk_norm_rope_append, rope_turns,
                     tree_attention, tree_commit)
+from .tree_decode import TreeDecoder, TreeStep
 from .quant import QuantizedWeight, pack_nibbles, quantize, unpack_nibbles
 
 __all__ = [
@@ -36,6 +37,8 @@ __all__ = [
     "unpack_nibbles",
     "PagedPlan",
     "TreeCommit",
+    "TreeDecoder",
+    "TreeStep",
     "paged_cache",
     "paged_plan",
     "qk_norm_rope_append",
