@@ -72,17 +72,21 @@ struct Shape {
   static constexpr int kKvBytes = kKeys * D * 2, kKvHalf = kKeys * 128; // a K or V tile
   static constexpr int kStages = D == 128 ? 5 : 10;                     // ring: 80 KB
   static constexpr int kSmem = kQBytes + kStages * kKvBytes;
-  // One partial: 128 rows of D values, maxima, sums.
+  // One partial: [D / 4][rows, up to a power of two][4] values (a warp, one row a lane, writes
+  // 512 bytes in a row), and from the 128 x D-th value on 128 maxima, 128 sums.
   static constexpr size_t kPartFloats = static_cast<size_t>(kTile) * (D + 2);
 };
 
-// What the joining kernel needs to know of a CTA.
-struct Meta {
-  int tail;       // an item begins in this CTA and goes on in the next: its partial is slot 1
-  int head_ends;  // the item of slot 0 ends in this CTA
-  int token, ntok, head;  // first token row, tokens and KV head of the slot 1 item
+// What the joining kernel needs to know of an item that lies in several CTAs: each of
+// them says so for itself, under the slot of its partial (rows 0: none).  Slot 1 holds the
+// part of an item that begins in the CTA, slot 0 of one that began before.
+struct alignas(16) Meta {
+  int rows, token, head;  // token: the first one's row
+  int first, parts;       // the CTAs that hold a part: [first, first + parts)
   int pad[3];
 };
+
+__device__ __forceinline__ int log2_up(int rows) { return 32 - __clz(rows - 1); }
 
 struct TreeAttnArgs {
   const uint16_t* q;
@@ -153,6 +157,8 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 // A CTA's way along the line.
 struct Walk {
   long long u, u1;  // next unit, end of the share
+  unsigned each;    // units of a share; the first `rest` shares have one more
+  int rest;
   int b, h, i0;     // item that u lies in: request, KV head, first token
   int off;          // units of it before u
   int loaded;       // whether r is request b's
@@ -434,6 +440,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
     Walk w;
     w.u = u0, w.u1 = u1, w.loaded = 1;
+    w.each = static_cast<unsigned>(min(each, 0xfffffff0ll)), w.rest = static_cast<int>(rest);
     long long o = u0 - before, hu = 0;
     for (w.b = b0;; ++w.b) {
       if (b1 - b0 > 1) req = load_request(p, w.b);
@@ -670,7 +677,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 
     bool more = next_item(0);
     if (more) load_q(item_at(0));
-    if (tid == 0) p.meta[blockIdx.x] = Meta{};
+    if (tid == 0) p.meta[2 * blockIdx.x] = p.meta[2 * blockIdx.x + 1] = Meta{};
     for (int k = 0; more; ++k) {
       const Item& it = item_at(k);
       const int n = it.hi - it.lo, lo = it.lo, full = it.full;
@@ -770,12 +777,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       // ---- the item's end
       const bool whole = lo == 0 && it.hi == it.nt;
       const int slot = lo > 0 ? 0 : 1;
-      if (!whole && tid == 0) {
-        Meta* mt = p.meta + blockIdx.x;
-        if (lo > 0)
-          mt->head_ends = it.hi == it.nt;
-        else
-          mt->tail = 1, mt->token = it.first + it.i0, mt->ntok = it.ntok, mt->head = it.h;
+      if (!whole && tid == 0) {  // the shares that hold the tiles before and after this one's
+        const unsigned each = sh->start.each;
+        const int c = blockIdx.x, rest = sh->start.rest;  // shares before `rest` have one unit more
+        auto shares = [&](unsigned tiles, int near, unsigned size, unsigned far) {  // `near` of one size, then others
+          const unsigned long long most = static_cast<unsigned long long>(near) * size;
+          return static_cast<int>(tiles <= most ? (tiles + size - 1) / size
+                                                : near + (tiles - static_cast<unsigned>(most) + far - 1) / far);
+        };
+        const int back = shares(lo, max(0, c - rest), each, each + 1);
+        const int ahead = shares(it.nt - it.hi, max(0, rest - c - 1), each + 1, each);
+        p.meta[2 * c + slot] = Meta{rows, it.first + it.i0, it.h, c - back, back + ahead + 1, {}};
       }
       ok = wait_warp(&sh->ofull, o_ph, p.err, abort);
       if (!ok) break;
@@ -818,9 +830,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
                                   pack_pair<BF16>(o[8 * q + 4], o[8 * q + 5]),
                                   pack_pair<BF16>(o[8 * q + 6], o[8 * q + 7]));
           } else {
-            float4* dst = reinterpret_cast<float4*>(part + static_cast<size_t>(row) * D + c);
+            const int lg = log2_up(rows);
+            float4* dst = reinterpret_cast<float4*>(part) + ((c / 4) << lg) + row;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            for (int q = 0; q < 8; ++q) dst[q << lg] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
           }
         }
         if (live) {
@@ -852,58 +865,77 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   }
 }
 
-// Joins the partials of the items that lie in several CTAs, in CTA order.  Block
-// (c, y): the item that begins in CTA c and goes on, rows y * kJoinRows on.
-constexpr int kJoinRows = 8, kJoinThreads = 256;
+// Joins the partials of the items that lie in several CTAs, in a fixed order.  One thread
+// has 8 values of a row, rows fastest, as the partials lie.  Block (c, y) works for one of
+// the two items that CTA c may hold a part of (y & 1): an item's elements are divided
+// evenly among the blocks of its CTAs, so that a few items of many parts keep all SMs busy and
+// no block is launched for nothing.  Many parts are shared by the warps of a block.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinFew = 2;
+
+// A softmax-weighted sum of 8 values: maximum, sum, values.
+struct Joined {
+  float m, l, v[8];
+  __device__ __forceinline__ void add(float m2, float l2, const float* v2) {
+    if (m2 == -INFINITY) return;
+    const float top = fmaxf(m, m2), f = exp2_approx(m - top), f2 = exp2_approx(m2 - top);
+    m = top;
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] * f + v2[i] * f2;
+  }
+};
 
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArgs p, int ctas) {
-  constexpr int kPer = D / 32;
+__global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArgs p) {
+  __shared__ float box[kJoinWarps][10][32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_next();
   pdl_wait_previous();
-  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Meta mt = p.meta[c];
-  if (!mt.tail) return;
-  const int rows = mt.ntok * p.G;
-  if (static_cast<int>(blockIdx.y) * kJoinRows >= rows) return;
-  int last = c + 1;  // the CTA in which the item ends
-  while (last < ctas - 1 && !p.meta[last].head_ends) ++last;
-  auto partial = [&](int cta) {
-    return p.part + (static_cast<size_t>(cta) * 2 + (cta == c ? 1 : 0)) * Shape<D>::kPartFloats;
-  };
-  for (int r = blockIdx.y * kJoinRows + warp; r < min(rows, static_cast<int>(blockIdx.y + 1) * kJoinRows);
-       r += kJoinThreads / 32) {
-    float top = -INFINITY;
-    for (int k = c + lane; k <= last; k += 32) top = fmaxf(top, partial(k)[kTile * D + r]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[kPer], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
-#pragma unroll 8
-    for (int k = c; k <= last; ++k) {
-      const float* src = partial(k);
-      const float m = src[kTile * D + r];
-      const float w = m == -INFINITY ? 0.f : exp2_approx(m - top);
-      sum += w * src[kTile * D + kTile + r];
-      if constexpr (kPer == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<size_t>(r) * D + lane * 4);
-        acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src + static_cast<size_t>(r) * D + lane * 2);
-        acc[0] += w * v.x, acc[1] += w * v.y;
+  const Meta mt = p.meta[2 * blockIdx.x + (blockIdx.y & 1)];
+  if (mt.rows == 0) return;
+  const bool many = mt.parts > kJoinFew;
+  const int lg = log2_up(mt.rows);
+  const int k0 = many ? warp : 0, step = many ? kJoinWarps : 1, pass = many ? 32 : kJoinThreads;
+  const int all = (D / 8) << lg, own = ((all + mt.parts - 1) / mt.parts + 31) & ~31;
+  const int begin = (blockIdx.x - mt.first) * own, end = min(all, begin + own);
+  const int e1 = begin + (blockIdx.y >> 1) * pass;
+  for (int e0 = e1; e0 < end; e0 += (gridDim.y >> 1) * pass) {
+    const int e = e0 + (many ? lane : tid), row = e & ((1 << lg) - 1), chunk = e >> lg;
+    const bool mine = row < mt.rows && e < end;
+    Joined j{-INFINITY, 0.f, {}};
+    if (mine) {
+#pragma unroll 4
+      for (int k = k0; k < mt.parts; k += step) {
+        const float* src = p.part + (static_cast<size_t>(mt.first + k) * 2 + (k == 0)) * Shape<D>::kPartFloats;
+        const float4* v = reinterpret_cast<const float4*>(src) + (chunk << (lg + 1)) + row;
+        const float4 a = v[0], b = v[1 << lg];
+        const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        j.add(src[kTile * D + row], src[kTile * D + kTile + row], w);
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const size_t row = static_cast<size_t>(mt.token + r / p.G) * p.Hq + mt.head * p.G + r % p.G;
-    uint32_t w[kPer / 2];
+    if (many) {
+      if (e0 != e1) __syncthreads();  // the box is free again
+      box[warp][0][lane] = j.m;
+      box[warp][1][lane] = j.l;
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j) w[j] = pack_pair<BF16>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-    if constexpr (kPer == 4)
-      *reinterpret_cast<uint2*>(p.out + row * D + lane * 4) = make_uint2(w[0], w[1]);
-    else
-      *reinterpret_cast<uint32_t*>(p.out + row * D + lane * 2) = w[0];
-    if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+      for (int i = 0; i < 8; ++i) box[warp][2 + i][lane] = j.v[i];
+      __syncthreads();
+      if (warp) continue;
+      for (int w = 1; w < kJoinWarps; ++w) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = box[w][2 + i][lane];
+        j.add(box[w][0][lane], box[w][1][lane], v);
+      }
+    }
+    if (!mine) continue;
+    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+    const int tk = row / p.G;
+    const size_t r = static_cast<size_t>(mt.token + tk) * p.Hq + mt.head * p.G + (row - tk * p.G);
+    *reinterpret_cast<uint4*>(p.out + r * D + chunk * 8) =
+        make_uint4(pack_pair<BF16>(j.v[0] * inv, j.v[1] * inv), pack_pair<BF16>(j.v[2] * inv, j.v[3] * inv),
+                   pack_pair<BF16>(j.v[4] * inv, j.v[5] * inv), pack_pair<BF16>(j.v[6] * inv, j.v[7] * inv));
+    if (p.lse && chunk == 0) p.lse[r] = j.l == 0.f ? -INFINITY : (j.m + log2f(j.l)) * 0.6931471805599453f;
   }
 }
 
@@ -943,9 +975,10 @@ int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAtt
   std::call_once(once[dev.device],
                  [&] { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
   if (int e = launch_chained(kern, dim3(ctas), dim3(kAttnThreads), smem, st, mk, mv, a)) return e;
+  // The shares of an item of 128 rows in two parts are 1024 elements; two passes each.
   const int rows = static_cast<int>(std::min<long long>(kTile, static_cast<long long>(a.T) * a.G));
-  return launch_chained(tree_attn_join<BF16, D>, dim3(ctas, (rows + kJoinRows - 1) / kJoinRows),
-                        dim3(kJoinThreads), 0, st, a, ctas);
+  return launch_chained(tree_attn_join<BF16, D>, dim3(ctas, 2 * ((rows * (D / 8) + 1023) / 1024)), dim3(kJoinThreads), 0, st,
+                        a);
 }
 
 }  // namespace
