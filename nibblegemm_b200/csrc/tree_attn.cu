@@ -69,7 +69,8 @@ template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
   static constexpr int kQBytes = kTile * D * 2, kQHalf = kTile * 128;   // a Q tile, its 64-value half
-  static constexpr int kKvBytes = kKeys * D * 2, kKvHalf = kKeys * 128; // a K or V tile
+  static constexpr int kKvBytes = kKeys * D * 2;                        // a K or V tile
+  static constexpr int kKvGroup = kHalves * 1024;                       // eight keys of it
   static constexpr int kStages = D == 128 ? 5 : 10;                     // ring: 80 KB
   static constexpr int kSmem = kQBytes + kStages * kKvBytes;
   // One partial: [D / 4][rows, up to a power of two][4] values (a warp, one row a lane, writes
@@ -86,6 +87,18 @@ struct alignas(16) Meta {
   int pad[3];
 };
 
+// How the TMA boxes lie in the cache.  A K or V tile is kept as [group of 8 keys][64-value
+// half][8 rows of 128 bytes], so that one box brings whole rows of a page (up to a tile)
+// wherever five dimensions can name them: 64 values, 8 rows, halves, groups, and a last
+// one that goes through heads and pages alike or has the heads joined to the halves.
+// Boxes of 16 rows x 128 bytes, one for each half, were issued too slowly: prompts of
+// 16-row pages took 384 us instead of 343.  Strides that no such view fits are read in
+// boxes of 8 rows and one half (split).
+struct BoxPlan {
+  int split;
+  int head2, page4, head4;  // third coordinate head * head2, fifth page * page4 + head * head4
+};
+
 __device__ __forceinline__ int log2_up(int rows) { return 32 - __clz(rows - 1); }
 
 struct TreeAttnArgs {
@@ -93,6 +106,7 @@ struct TreeAttnArgs {
   long long q_token, q_head;
   const uint16_t* v;
   CacheStrides cs;
+  BoxPlan box;
   const int* table;
   long long table_stride;
   int table_width;
@@ -218,12 +232,12 @@ struct alignas(16) Shared {
 // ---------------------------------------------------------------------------
 // PTX used here only
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint64_t* bar, int c0, int c1,
-                                            int c2, int c3) {
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3, int c4) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -242,16 +256,14 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // Shared-memory matrix descriptors, low words (start address >> 4, leading offset
-// >> 4 from bit 16) and the high word that both kinds share: stride offset 1024 B
-// (eight 128-byte rows), version 1, 128-byte swizzle.
+// >> 4 from bit 16) and high words: stride offset (to the next eight 128-byte rows),
+// version 1, 128-byte swizzle.
 //   K-major (Q, K): rows of 64 values; the leading offset is not used.
 //   N-major (V as the B operand, N = the D values contiguous): 8 keys per atom, the
 //   stride offset steps along the keys, the leading offset to the next 64 values.
-constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t desc_high(int stride) { return (stride >> 4) | (1u << 14) | (2u << 29); }
 __device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr, uint32_t half_bytes) {
-  return (addr >> 4) | ((half_bytes >> 4) << 16);
-}
+__device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr) { return (addr >> 4) | ((1024u >> 4) << 16); }
 
 // Keeps the compiler from computing the operands of all products of an item ahead
 // of its loop, which takes more registers than the warp has.
@@ -260,20 +272,22 @@ __device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b, uint32_t& c) {
 }
 
 // D[tmem] (+)= A * B, descriptors by their low words; A from shared / from tensor memory.
+template <int D>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .b64 x, y;\n\t.reg .pred p;\n\t"
-      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(accumulate)
+      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "n"(desc_high(1024)), "n"(desc_high(Shape<D>::kKvGroup)), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+template <int D>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .b64 y;\n\t.reg .pred p;\n\t"
       "mov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(accumulate)
+      "r"(a), "r"(b), "n"(desc_high(Shape<D>::kKvGroup)), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -483,11 +497,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   // Places of the ring in an item of n tiles: K0 K1 V0 K2 V1 K3 ..., the order of the MMAs.
   if (warp == 4) {
     // ------------------------------------------------------------ TMA producer
-    const int shift = min(p.page_shift, 6);  // rows of a piece: a page, or a whole tile of one
-    const int pieces = kKeys >> shift;
-    const int piece = lane % pieces, half = lane / pieces;
-    const uint32_t piece_bytes = 128u << shift;
-    const uint32_t offset = half * Sh::kKvHalf + piece * piece_bytes;
+    const BoxPlan box = p.box;
+    const int shift = box.split ? 3 : min(p.page_shift, 6);  // rows of a box: a page, or a whole tile of one
+    const int pieces = kKeys >> shift, halves = box.split ? Sh::kHalves : 1;
+    const int piece = lane / halves, half = lane % halves;
+    const uint32_t piece_bytes = (box.split ? 128u : 2u * D) << shift;
+    const uint32_t offset = lane * piece_bytes;
     const int page_mask = (1 << p.page_shift) - 1;
     uint32_t st = 0, ph = 0;  // stage and parity of the next place
     bool ok = true;
@@ -505,7 +520,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const int n = it.hi - it.lo;
       const int* row = p.table + static_cast<long long>(it.b) * p.table_stride;
       auto key_at = [&](int j) { return (it.lo + j) * kKeys + (piece << shift); };
-      auto active_at = [&](int j) { return half < Sh::kHalves && j < n && key_at(j) < it.need; };
+      auto active_at = [&](int j) { return piece < pieces && j < n && key_at(j) < it.need; };
       auto page_at = [&](int j) { return active_at(j) ? row[key_at(j) >> p.page_shift] : 0; };
       auto load = [&](bool is_v, int j, int page) {
         if (!wait_warp(&sh->empty[st], ph ^ 1, p.err, abort)) return false;
@@ -518,8 +533,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             atomicOr(p.err, kErrBadIndex);
             page = p.num_pages;
           }
-          tma_load_4d(smem_u32(ring + st * Sh::kKvBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[st],
-                      half * 64, key_at(j) & page_mask, it.h, page);
+          const int at = key_at(j) & page_mask;
+          tma_load_5d(smem_u32(ring + st * Sh::kKvBytes) + offset, is_v ? &tmap_v : &tmap_k, &sh->full[st], 0,
+                      box.split ? at : 0, box.split ? half : it.h * box.head2, box.split ? it.h : at >> 3,
+                      page * box.page4 + it.h * box.head4);
         }
         if (++st == kStages) st = 0, ph ^= 1;
         return true;
@@ -543,7 +560,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t q_desc = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(smem)), 0);
     const uint32_t ring_k = __shfl_sync(0xffffffffu, desc_kmajor(smem_u32(ring)), 0);
-    const uint32_t ring_v = __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring), Sh::kKvHalf), 0);
+    const uint32_t ring_v = __shfl_sync(0xffffffffu, desc_nmajor(smem_u32(ring)), 0);
     auto advance = [&]() {
       if (++st == kStages) st = 0, ph ^= 1;
     };
@@ -555,8 +572,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         opaque(d, qd, kd);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          mma_ss(d, qd + (((kk >> 2) * Sh::kQHalf + (kk & 3) * 32) >> 4),
-                 kd + (((kk >> 2) * Sh::kKvHalf + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
+          mma_ss<D>(d, qd + (((kk >> 2) * Sh::kQHalf + (kk & 3) * 32) >> 4),
+                 kd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
         umma_commit(&sh->sfull[b]);
         umma_commit(&sh->empty[st]);
       }
@@ -583,7 +600,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           opaque(d, a, vd);
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(j != 0));
+            mma_ts<D>(d, a + kk * 8, vd + kk * (2 * Sh::kKvGroup >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(j != 0));
           umma_commit(&sh->empty[st]);
           if (j == n - 2) umma_commit(&sh->olast);
           if (j == n - 1) umma_commit(&sh->ofull);
@@ -622,7 +639,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll
         for (int q = 0; q < D / 16; ++q) {
           const int c = q * 2 + (tid & 1);  // 16-byte chunk of the row
-          uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * Sh::kKvHalf + r * 128 + (((c + r) & 7) << 4));
+          uint4* at = reinterpret_cast<uint4*>(tile + (r >> 3) * Sh::kKvGroup + (c >> 3) * 1024 + (r & 7) * 128 + (((c + r) & 7) << 4));
           if (beyond) {
             *at = make_uint4(0, 0, 0, 0);
             continue;
@@ -942,16 +959,35 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-int make_cache_map(const void* base, const CacheStrides& cs, int D, int rows, int Hkv, int pages, CUtensorMap* m) {
+BoxPlan plan_boxes(const CacheStrides& cs, int D, int Hkv, int pages) {
+  if (D == 64) return {0, 1, 1, 0};
+  if (cs.head == D || Hkv == 1) return {0, 2, 1, 0};         // a row of all heads is one run of halves
+  if (cs.page == cs.head * Hkv && static_cast<long long>(pages) * Hkv < (1LL << 31))
+    return {0, 0, Hkv, 1};                                   // heads go on from page to page
+  return {1, 0, 1, 0};
+}
+
+int make_cache_map(const void* base, const CacheStrides& cs, const BoxPlan& plan, int D, int rows, int Hkv, int pages,
+                   CUtensorMap* m) {
   auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode_fn());
   if (!enc) return NG_ERR_CUDA;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows),
-                              static_cast<cuuint64_t>(Hkv), static_cast<cuuint64_t>(pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(cs.row) * 2, static_cast<cuuint64_t>(cs.head) * 2,
-                                 static_cast<cuuint64_t>(cs.page) * 2};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(rows, kKeys)), 1, 1};
-  const cuuint32_t es[4] = {1, 1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, es,
+  const cuuint64_t u = 2, heads = Hkv, groups = rows / 8;
+  const cuuint64_t row = cs.row * u, head = cs.head * u, page = cs.page * u;
+  const cuuint32_t halves = D / 64, most = std::min(rows, kKeys) / 8;
+  cuuint64_t dims[5] = {64, 8, halves, groups, static_cast<cuuint64_t>(pages)};
+  cuuint64_t strides[4] = {row, 128, 8 * row, page};
+  cuuint32_t box[5] = {64, 8, halves, most, 1};
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  if (plan.split) {
+    dims[1] = rows, dims[3] = heads, strides[2] = head;
+    box[2] = box[3] = 1;
+  } else if (plan.head4) {
+    dims[4] *= heads, strides[3] = head;
+  } else {
+    dims[2] *= heads;
+    if (halves == 1) strides[1] = head;
+  }
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, const_cast<void*>(base), dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? NG_OK
@@ -1018,11 +1054,12 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
   if (int st = current_device_info(&dev)) return st;
   if (workspace_bytes < attn_workspace_bytes(D, dev)) return NG_ERR_BAD_ARGUMENT;
   CUtensorMap mk, mv;
-  if (int st = make_cache_map(k_cache, cs, D, page_size, Hkv, num_pages, &mk)) return st;
-  if (int st = make_cache_map(v_cache, cs, D, page_size, Hkv, num_pages, &mv)) return st;
+  const BoxPlan box = plan_boxes(cs, D, Hkv, num_pages);
+  if (int st = make_cache_map(k_cache, cs, box, D, page_size, Hkv, num_pages, &mk)) return st;
+  if (int st = make_cache_map(v_cache, cs, box, D, page_size, Hkv, num_pages, &mv)) return st;
   const int G = Hq / Hkv;
   const TreeAttnArgs a{static_cast<const uint16_t*>(q), q_stride_token, q_stride_head,
-                       static_cast<const uint16_t*>(v_cache), cs, block_table, table_stride, table_width, kv_lens,
+                       static_cast<const uint16_t*>(v_cache), cs, box, block_table, table_stride, table_width, kv_lens,
                        cu_new, reinterpret_cast<const unsigned long long*>(mask), mask_words,
                        static_cast<uint16_t*>(out), lse, B, T, Hq, Hkv, G, kTile / G, num_pages,
                        log2_of(page_size), scale * 1.4426950408889634f,
