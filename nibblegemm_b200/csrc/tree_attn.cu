@@ -11,9 +11,9 @@
 //
 // Two persistent CTAs per SM, each warp-specialised:
 //   warps 0-3  softmax, one thread per row
-//   warp 4     walks this CTA's share of the work and hands out its items; TMA: the
-//              pages of a K or V tile into a ring of stages, one lane per page and
-//              64-value half, 128-byte swizzle
+//   warp 4     walks this CTA's share of the work and hands out its items; TMA: an
+//              item's Q, and the pages of a K or V tile into a ring of stages, one lane
+//              per box, 128-byte swizzle
 //   warp 5     tcgen05.mma: S = Q K^T (128 x 64, both operands from shared
 //              memory), O += P V (P from tensor memory)
 // Tensor memory: two buffers of scores (64 columns each; P is written over the
@@ -109,8 +109,6 @@ struct BoxPlan {
 __device__ __forceinline__ int log2_up(int rows) { return 32 - __clz(rows - 1); }
 
 struct TreeAttnArgs {
-  const uint16_t* q;
-  long long q_token, q_head;
   const uint16_t* v;
   CacheStrides cs;
   BoxPlan box;
@@ -257,7 +255,8 @@ template <int kStages, bool kPairs>
 struct alignas(16) Shared {
   uint64_t full[kStages], empty[kStages];
   uint64_t sfull[2], pfull[2];  // by buffer
-  uint64_t qfull, ofull, olast; // olast: all but the last P V of an item are done
+  uint64_t qfull, qempty;       // Q is there; the item's last scores are computed
+  uint64_t ofull, olast;        // olast: all but the last P V of an item are done
   uint64_t item_full[kItems], item_empty[kItems];
   Item items[kItems];
   long long warp_sum[2][kAttnThreads / 32];
@@ -276,6 +275,14 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, uint
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -421,6 +428,7 @@ __device__ __forceinline__ uint32_t visible(const TreeAttnArgs& p, const Item& i
 template <bool BF16, int D, bool kPairs>
 __global__ void __launch_bounds__(kAttnThreads, 2)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                     const __grid_constant__ CUtensorMap tmap_tile, const __grid_constant__ CUtensorMap tmap_token,
                      const __grid_constant__ TreeAttnArgs p) {
   using Sh = Shape<D>;
   constexpr int kStages = Sh::kStages, kFirst = kPairs ? 0 : 1;  // kFirst: the first line
@@ -439,7 +447,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       mbar_init(&sh->sfull[b], 1);
       mbar_init(&sh->pfull[b], 4);
     }
-    mbar_init(&sh->qfull, 4);
+    mbar_init(&sh->qfull, 1);
+    mbar_init(&sh->qempty, 1);
     mbar_init(&sh->ofull, 1);
     mbar_init(&sh->olast, 1);
     for (int s = 0; s < kItems; ++s) {
@@ -453,8 +462,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     mbar_fence_init();
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
+    tma_prefetch_desc(&tmap_token);
   }
   if (warp == 5) tmem_alloc(&sh->tmem, 256);
+  for (int c = tid; c < Sh::kQBytes / 16; c += kAttnThreads) reinterpret_cast<uint4*>(smem)[c] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   pdl_launch_next();
   pdl_wait_previous();
 
@@ -551,6 +563,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const uint32_t offset = lane * piece_bytes;
     const int page_mask = (1 << p.page_shift) - 1;
     uint32_t st = 0, ph = 0;  // stage and parity of the next place
+    int filled = 0;           // rows of Q in shared memory that may not be zero
     bool ok = true;
     Walk<kPairs> walk = sh->start[kFirst];
     for (int k = 0; ok; ++k) {
@@ -587,8 +600,32 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         if (++st == kStages) st = 0, ph ^= 1;
         return true;
       };
+      // The item's Q rows, a box for a whole tile or one for each token, and zeros in the rows
+      // beyond: products with zero take a fraction of the power, and under the power limit
+      // of a long decode that is clock rate (64 x 8192 single tokens of 4 rows: 242 -> 224 us).
+      // (Loaded by the softmax warps, Q took 2000 to 7000 cycles of an item: 1000 contexts of up
+      // to 500 rows 357 us instead of 272.)
+      auto load_q = [&]() {
+        if (!wait_warp(&sh->qempty, (k & 1) ^ 1, p.err, abort)) return false;
+        const int rows = it.ntok * p.G;
+        for (int c = rows * (D / 8) + lane; c < filled * (D / 8); c += 32)
+          *reinterpret_cast<uint4*>(smem + (c & 7) * 16 + (c >> 3) % Sh::kHalves * Sh::kQHalf +
+                                    (c >> 3) / Sh::kHalves * 128) = make_uint4(0, 0, 0, 0);
+        filled = rows;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&sh->qfull, rows * D * 2);
+        __syncwarp();
+        const bool tile = it.ntok == p.tok_tile;
+        for (int i = lane; i < (tile ? 1 : it.ntok) * Sh::kHalves; i += 32) {
+          const int h = i % Sh::kHalves, tk = i / Sh::kHalves;
+          tma_load_3d(smem_u32(smem) + h * Sh::kQHalf + tk * p.G * 128, tile ? &tmap_tile : &tmap_token, &sh->qfull,
+                      h * 64, it.h * p.G, it.first + it.i0 + tk);
+        }
+        return true;
+      };
       int pg0 = page_at(0), pg1 = page_at(1);  // of tiles j and j + 1
-      ok = load(false, 0, pg0) && (n == 1 || load(false, 1, pg1));
+      ok = load(false, 0, pg0) && load_q() && (n == 1 || load(false, 1, pg1));
       for (int j = 0; ok && j < n; ++j) {
         const int pg2 = page_at(j + 2);
         ok = load(true, j, pg0) && (j + 2 >= n || load(false, j + 2, pg2));
@@ -610,7 +647,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     auto advance = [&]() {
       if (++st == kStages) st = 0, ph ^= 1;
     };
-    auto scores = [&](int b) {  // S = Q K^T into buffer b, K at the current place
+    auto scores = [&](int b, bool last) {  // S = Q K^T into buffer b, K at the current place
       if (!wait_warp(&sh->full[st], ph, p.err, abort)) return false;
       tc_fence_after();
       if (elect_one()) {
@@ -621,6 +658,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           mma_ss<D>(d, qd + (((kk >> 2) * Sh::kQHalf + (kk & 3) * 32) >> 4),
                  kd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), idesc_s, kk != 0);
         umma_commit(&sh->sfull[b]);
+        if (last) umma_commit(&sh->qempty);
         umma_commit(&sh->empty[st]);
       }
       __syncwarp();
@@ -634,7 +672,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (lane == 0) done(k);
       ok = wait_warp(&sh->qfull, q_ph, p.err, abort);
       q_ph ^= 1;
-      ok = ok && scores(0) && (n == 1 || scores(1));
+      ok = ok && scores(0, n == 1) && (n == 1 || scores(1, n == 2));
       for (int j = 0; ok && j < n; ++j) {  // O += P V of tile j, then the scores of tile j + 2
         const int b = j & 1;
         ok = wait_warp(&sh->full[st], ph, p.err, abort) && wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort);
@@ -653,7 +691,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         }
         __syncwarp();
         advance();
-        if (j + 2 < n) ok = scores(b);
+        if (j + 2 < n) ok = scores(b, j + 3 == n);
       }
     }
   } else {
@@ -663,7 +701,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const uint32_t ts = tmem + lanes, to = tmem + 2 * kKeys + lanes;  // scores, O
     uint32_t s_ph = 0, o_ph = 0, last_ph = 0;  // parities: S (bit buffer), O, olast
     uint32_t places = 0;                       // ring places of the items before
-    int filled = kTile;                        // rows of Q in shared memory that may not be zero
     bool ok = true;
     const int rt = row / p.G;
 
@@ -707,39 +744,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       fence_proxy_async_smem();
     };
 
-    // The item's Q rows into shared memory (128-byte swizzle), zeros in the rows beyond:
-    // products with zero take a fraction of the power, and under the power limit
-    // of a long decode that is clock rate (64 x 8192 single tokens of 4 rows: 242 -> 224 us).
-    auto load_q = [&](const Item& x) {
-      const int rows = x.ntok * p.G;
-      constexpr int kChunks = D / 8, kStep = kTile / kChunks;  // a thread: one chunk of every kStep-th row
-      const int c = row % kChunks, r0 = row / kChunks;
-      const uint16_t* src = p.q + static_cast<long long>(x.first + x.i0) * p.q_token +
-                            static_cast<long long>(x.h) * p.G * p.q_head + c * 8;
-      unsigned char* dst = smem + (c >> 3) * Sh::kQHalf;
-      const int fill = max(rows, filled);  // rows that must be written: the item's, the ones in use before
-      filled = rows;
-      for (int rr = r0; rr < fill; rr += 8 * kStep) {  // eight loads in flight
-        uint4 v[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int r = rr + q * kStep, tk = r / p.G;
-          v[q] = make_uint4(0, 0, 0, 0);
-          if (r < rows) v[q] = ld_ro_v4(src + tk * p.q_token + (r - tk * p.G) * p.q_head);
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int r = rr + q * kStep;
-          if (r < fill) *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[q];
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->qfull);
-    };
-
     bool more = next_item(0);
-    if (more) load_q(item_at(0));
     // Where the partials and their descriptions lie: the shares of the even tiles, of the
     // odd ones, of the line of single tiles.
     const int place0 = (blockIdx.x & 1) * (gridDim.x / 2) + blockIdx.x / 2, place1 = 2 * gridDim.x - 1 - blockIdx.x;
@@ -839,7 +844,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (!ok) break;
       places += 2 * n;
       more = next_item(k + 1);
-      if (more) load_q(item_at(k + 1));
 
       // ---- the item's end
       const bool whole = lo == 0 && it.hi == it.nt;
@@ -1051,6 +1055,21 @@ int make_cache_map(const void* base, const CacheStrides& cs, const BoxPlan& plan
              : NG_ERR_CUDA;
 }
 
+// Q, in boxes of `tokens` tokens of one KV head's query heads.
+int make_q_map(const void* base, long long token, long long head, int D, int Hq, int T, int G, int tokens, CUtensorMap* m) {
+  auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode_fn());
+  if (!enc) return NG_ERR_CUDA;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(Hq > 1 ? head : D) * 2, static_cast<cuuint64_t>(T > 1 ? token : D) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(tokens)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? NG_OK
+             : NG_ERR_CUDA;
+}
+
 constexpr size_t kMetaBytes = 65536;
 size_t attn_workspace_bytes(int D, const DeviceInfo& dev) {
   const size_t part = D == 128 ? Shape<128>::kPartFloats : Shape<64>::kPartFloats;
@@ -1058,7 +1077,8 @@ size_t attn_workspace_bytes(int D, const DeviceInfo& dev) {
 }
 
 template <bool BF16, int D, bool kPairs>
-int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnArgs& a, const DeviceInfo& dev,
+int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mtile, const CUtensorMap& mtoken,
+                     const TreeAttnArgs& a, const DeviceInfo& dev,
                      cudaStream_t st) {
   constexpr int smem = Shape<D>::kSmem + static_cast<int>(sizeof(Shared<Shape<D>::kStages, kPairs>));
   static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs must fit in the shared memory of an SM");
@@ -1067,7 +1087,7 @@ int launch_tree_attn(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAtt
   static std::once_flag once[kMaxDevices];
   std::call_once(once[dev.device],
                  [&] { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-  if (int e = launch_chained(kern, dim3(ctas), dim3(kAttnThreads), smem, st, mk, mv, a)) return e;
+  if (int e = launch_chained(kern, dim3(ctas), dim3(kAttnThreads), smem, st, mk, mv, mtile, mtoken, a)) return e;
   // The shares of an item of 128 rows in two parts are 1024 elements; two passes each.
   const int rows = static_cast<int>(std::min<long long>(kTile, static_cast<long long>(a.T) * a.G));
   return launch_chained(tree_attn_join<BF16, D, kPairs>, dim3(ctas, 2 * ((rows * (D / 8) + 1023) / 1024)), dim3(kJoinThreads), 0, st,
@@ -1110,13 +1130,14 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
   DeviceInfo dev;
   if (int st = current_device_info(&dev)) return st;
   if (workspace_bytes < attn_workspace_bytes(D, dev)) return NG_ERR_BAD_ARGUMENT;
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mtile, mtoken;
   const BoxPlan box = plan_boxes(cs, D, Hkv, num_pages);
   if (int st = make_cache_map(k_cache, cs, box, D, page_size, Hkv, num_pages, &mk)) return st;
   if (int st = make_cache_map(v_cache, cs, box, D, page_size, Hkv, num_pages, &mv)) return st;
   const int G = Hq / Hkv;
-  const TreeAttnArgs a{static_cast<const uint16_t*>(q), q_stride_token, q_stride_head,
-                       static_cast<const uint16_t*>(v_cache), cs, box, block_table, table_stride, table_width, kv_lens,
+  if (int st = make_q_map(q, q_stride_token, q_stride_head, D, Hq, T, G, kTile / G, &mtile)) return st;
+  if (int st = make_q_map(q, q_stride_token, q_stride_head, D, Hq, T, G, 1, &mtoken)) return st;
+  const TreeAttnArgs a{static_cast<const uint16_t*>(v_cache), cs, box, block_table, table_stride, table_width, kv_lens,
                        cu_new, reinterpret_cast<const unsigned long long*>(mask), mask_words,
                        static_cast<uint16_t*>(out), lse, B, T, Hq, Hkv, G, kTile / G, num_pages,
                        log2_of(page_size), scale * 1.4426950408889634f,
@@ -1126,8 +1147,8 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
   // As many tokens as one tile holds: no request has two tiles, and the kernel without the
   // line of pairs starts sooner (one token, 777 rows: 12.3 us instead of 12.8).
   auto launch = [&](auto bf16, auto dim) {
-    return T <= a.tok_tile ? launch_tree_attn<bf16.value, dim.value, false>(mk, mv, a, dev, st)
-                           : launch_tree_attn<bf16.value, dim.value, true>(mk, mv, a, dev, st);
+    return T <= a.tok_tile ? launch_tree_attn<bf16.value, dim.value, false>(mk, mv, mtile, mtoken, a, dev, st)
+                           : launch_tree_attn<bf16.value, dim.value, true>(mk, mv, mtile, mtoken, a, dev, st);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
