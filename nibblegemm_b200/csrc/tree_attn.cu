@@ -59,8 +59,13 @@ constexpr int kKeys = 64;          // keys of a key tile
 constexpr int kAttnThreads = 192;  // 6 warps; two CTAs an SM leave 168 registers a thread
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
 constexpr int kItems = 4;          // work items handed out ahead
-constexpr int kMinUnits = 4;       // least work of a CTA, in key tiles
-constexpr int kItemUnits = 4;      // what an item costs beside its key tiles, in key tiles
+// Least work of a CTA, in key tiles: few requests are spread wide, but not so that most
+// of a CTA's time is its start (one token: 777 rows 12.3 us with 4, 11.5 with 2, 11.2 with 1;
+// 4000 rows 13.9, 13.0 and 14.9; a tree of 60 over 2000 rows 24.6, 21.7 and 21.6).
+constexpr int kMinUnits = 2;
+// What an item costs beside its key tiles, in key tiles (32 trees: 108 us with 1, 104.8 with 4,
+// 104.2 with 6; 1000 short contexts 280, 275 and 276).
+constexpr int kItemUnits = 4;
 
 // A work item as one CTA sees it.
 struct alignas(16) Item {
