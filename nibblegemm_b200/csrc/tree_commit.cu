@@ -16,6 +16,9 @@
 // (an atomic minimum, whose order does not matter), and the path is a chase through shared
 // memory: two rounds of global loads instead of two for every node of the path.
 // Trees of more nodes than fit there are walked with a ballot over the children.
+//
+// Bound: latency for few trees (4 of 32 nodes, 32 layers: 3.8 us on a B200), then HBM (64
+// of them: 7.4 us; the 50 MB that move would take 7.7 us from HBM, part of them is in L2).
 #include <algorithm>
 
 #include "paged_common.cuh"
