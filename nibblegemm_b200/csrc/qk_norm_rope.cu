@@ -19,9 +19,10 @@
 //
 // Bound: HBM for many tokens.  Four rows are loaded ahead (with one, the loads
 // of a warp were exposed one after another: 56 us where four take 40; two, three and six
-// are slower).  8192 tokens of 48 rows of 128, bf16, on a B200: 39.5 us, 5.1 TB/s;
-// 976 tokens of 80 rows 12.4 us, too few warps to cover the latency of their loads; 4 tokens
-// 2.2 us, the launch.
+// are slower).  128 registers a thread, 16 warps an SM (20 of 96: 2000 tokens of 48 rows
+// 14.0 us, not 11.7).  8192 tokens of 48 rows of 128, bf16, on a B200: 38.9 us, 5.2 TB/s;
+// 976 tokens of 80 rows 10.7 us, one round of loads after another; 4 tokens 2.2 us, the
+// launch.
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -30,6 +31,7 @@ namespace ngb {
 namespace {
 
 constexpr int kNrThreads = 128;
+constexpr int kNrBlocks = 4;  // blocks an SM: 128 registers a thread
 
 struct NormRopeArgs {
   const uint16_t* qkv;
@@ -43,14 +45,15 @@ struct NormRopeArgs {
   uint16_t* k_cache;
   uint16_t* v_cache;
   CacheStrides cs;
-  int M, Hq, Hkv, rot, page_shift, chunks;
+  int M, Hq, Hkv, rot, page_shift;
+  int whole, chunks;  // tokens that one warp takes each; warps for each of the others
   long long num_rows;  // pages * page size
   float eps;
   unsigned int* err;
 };
 
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const NormRopeArgs p) {
+__global__ void __launch_bounds__(kNrThreads, kNrBlocks) qk_norm_rope_kernel(const NormRopeArgs p) {
   constexpr int kLanes = D / 8;        // lanes per row
   constexpr int kRows = 32 / kLanes;   // rows per warp and step
   constexpr int kAhead = 4;            // steps whose rows are loaded together
@@ -58,12 +61,13 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const NormRope
   pdl_wait_previous();
   const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
   const int gw = blockIdx.x * (kNrThreads / 32) + (threadIdx.x >> 5);
-  const int m = gw / p.chunks, chunk = gw % p.chunks;
+  const int chunks = gw < p.whole ? 1 : p.chunks, rest = gw - p.whole;
+  const int m = gw < p.whole ? gw : p.whole + rest / chunks, chunk = gw < p.whole ? 0 : rest % chunks;
   if (m >= p.M) return;
   // Steps of the three sections, and this warp's run of them.
   const int q_steps = (p.Hq + kRows - 1) / kRows, k_steps = (p.Hkv + kRows - 1) / kRows;
   const int steps = q_steps + 2 * k_steps;
-  const int s0 = steps * chunk / p.chunks, s1 = steps * (chunk + 1) / p.chunks;
+  const int s0 = steps * chunk / chunks, s1 = steps * (chunk + 1) / chunks;
 
   const uint16_t* src = p.qkv + static_cast<size_t>(m) * p.qkv_stride + l * 8;
   const int slot = p.slots[m];
@@ -205,11 +209,16 @@ template <bool BF16, int D>
 int launch_norm_rope(NormRopeArgs a, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int kRows = 256 / D;
   const int steps = (a.Hq + kRows - 1) / kRows + 2 * ((a.Hkv + kRows - 1) / kRows);
-  // Few tokens: one step a warp, to spread the rows over the SMs.  Many: one
-  // warp a token, so the sines are computed once.
-  const long long want = static_cast<long long>(dev.sm_count) * 32;
-  a.chunks = static_cast<int>(std::max<long long>(1, std::min<long long>(steps, want / a.M)));
-  const long long warps = static_cast<long long>(a.M) * a.chunks;
+  // A warp that has a whole token works out its sines once, so as many tokens as fill the SMs
+  // a whole number of times go to a warp each.  Those that are left over are shared by as
+  // many warps as the SMs hold at once, but no more: 976 tokens of 80 rows take 10.7 us with
+  // two warps a token, 13.2 with four, of which some wait for the others; 2500 of 48 rows
+  // 19.1 us with a warp for every token, and 14.7 so.
+  const int wave = dev.sm_count * kNrBlocks * (kNrThreads / 32);
+  a.whole = a.M / wave * wave;
+  const int rest = a.M - a.whole;
+  a.chunks = rest ? std::min(steps, wave / rest) : 1;
+  const long long warps = a.whole + static_cast<long long>(rest) * a.chunks;
   const long long blocks = (warps + kNrThreads / 32 - 1) / (kNrThreads / 32);
   return launch_chained(qk_norm_rope_kernel<BF16, D>, dim3(static_cast<unsigned>(blocks)), dim3(kNrThreads), 0,
                         st, a);
@@ -243,7 +252,7 @@ extern "C" int ng_qk_norm_rope_append(const void* qkv, long long qkv_stride, con
   const NormRopeArgs a{static_cast<const uint16_t*>(qkv), qkv_stride, static_cast<const uint16_t*>(q_weight),
                        static_cast<const uint16_t*>(k_weight), turns, positions, slots,
                        static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_cache),
-                       static_cast<uint16_t*>(v_cache), cs, M, Hq, Hkv, rotary_dim, log2_of(page_size), 1,
+                       static_cast<uint16_t*>(v_cache), cs, M, Hq, Hkv, rotary_dim, log2_of(page_size), 0, 1,
                        static_cast<long long>(num_pages) * page_size, eps, dev.err};
   auto st = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == NG_DTYPE_BF16;
