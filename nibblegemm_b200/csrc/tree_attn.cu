@@ -195,6 +195,7 @@ __device__ __forceinline__ long long head_units(const TreeAttnArgs& p, const Req
   if (p.mask || s.end - s.begin == s.stride)
     return static_cast<long long>((s.end - s.begin) / s.stride) * place_units(p, r, s.begin, s.stride);
   long long u = 0;
+#pragma unroll 1
   for (int i0 = s.begin; i0 < s.end; i0 += s.stride) u += place_units(p, r, i0, s.stride);
   return u;
 }
@@ -373,6 +374,10 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+template <bool BF16>
+__device__ __forceinline__ float value(uint16_t v) {
+  return BF16 ? __uint_as_float(static_cast<uint32_t>(v) << 16) : __half2float(__ushort_as_half(v));
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -387,6 +392,14 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
 // Bounded wait; false once the CTA has given up.  Plain polling measured fastest: a
 // suspend-time hint or a nanosleep between polls adds its wake-up to a chain of short
 // hand-overs (one token, 777 rows: 12.8 us as it is, 14 and more with either).
+// Kept short, as there are many of them: one place that polls, and the low word of the timer
+// (nanoseconds; it wraps after four seconds).  Reading it also paces the polls: with the
+// clock instead the waiting warps took issue slots from the others (chains 357 us, 340 so).
+__device__ __forceinline__ uint32_t timer_ns() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned int* err, volatile int* abort) {
   auto poll = [&]() {
     uint32_t ok;
@@ -400,16 +413,14 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigne
     return ok != 0;
   };
   if (poll()) return true;
-  const uint64_t t0 = global_timer_ns();
+  const uint32_t t0 = timer_ns();
   for (;;) {
     if (poll()) return true;
-    if (*abort) return false;
-    if (global_timer_ns() - t0 > 1000000000ull) {
-      atomicOr(err, kErrWaitTimeout);
-      *abort = 1;
-      return false;
-    }
+    if (*abort || timer_ns() - t0 > 1000000000u) break;
   }
+  atomicOr(err, kErrWaitTimeout);
+  *abort = 1;
+  return false;
 }
 // The same for a converged warp.  All lanes poll: one lane's answer would have to be
 // passed to the others first.
@@ -479,6 +490,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     tma_prefetch_desc(&tmap_token);
   }
   if (warp == 5) tmem_alloc(&sh->tmem, 256);
+#pragma unroll 1
   for (int c = tid; c < Sh::kQBytes / 16; c += kAttnThreads) reinterpret_cast<uint4*>(smem)[c] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   pdl_launch_next();
@@ -490,6 +502,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   const int tokens = min(max(p.cu[p.B], 0), p.T);
   long long mine[2] = {0, 0};
   Request req = {0, 0, 0, 0};
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     req = load_request(p, b);
 #pragma unroll
@@ -529,6 +542,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       w.u = u0, w.u1 = u1, w.loaded = 1, w.line = l, w.share = share;
       w.each = static_cast<unsigned>(min(each, 0xfffffff0ll)), w.rest = static_cast<int>(rest);
       long long o = u0 - before, hu = 0;
+#pragma unroll 1
       for (w.b = b0;; ++w.b) {
         if (b1 - b0 > 1) req = load_request(p, w.b);
         w.s = stretch<kPairs>(p, req, l);
@@ -539,6 +553,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       w.r = req;
       w.h = static_cast<int>(quotient(o, hu));
       o -= w.h * hu;
+#pragma unroll 1
       for (w.i0 = w.s.begin;; w.i0 += w.s.stride) {
         const int units = place_units(p, req, w.i0, w.s.stride);
         if (o < units) break;
@@ -550,6 +565,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   }
   __syncthreads();
   // rows beyond the last request's tokens see nothing
+#pragma unroll 1
   for (long long i = static_cast<long long>(tokens) * p.Hq * (D / 8) +
                      static_cast<long long>(blockIdx.x) * kAttnThreads + tid;
        i < static_cast<long long>(p.T) * p.Hq * (D / 8); i += static_cast<long long>(gridDim.x) * kAttnThreads) {
@@ -622,6 +638,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       auto load_q = [&]() {
         if (!wait_warp(&sh->qempty, (k & 1) ^ 1, p.err, abort)) return false;
         const int rows = it.ntok * p.G;
+#pragma unroll 1
         for (int c = rows * (D / 8) + lane; c < filled * (D / 8); c += 32)
           *reinterpret_cast<uint4*>(smem + (c & 7) * 16 + (c >> 3) % Sh::kHalves * Sh::kQHalf +
                                     (c >> 3) / Sh::kHalves * 128) = make_uint4(0, 0, 0, 0);
@@ -631,6 +648,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         if (lane == 0) mbar_arrive_expect_tx(&sh->qfull, rows * D * 2);
         __syncwarp();
         const bool tile = it.ntok == p.tok_tile;
+#pragma unroll 1
         for (int i = lane; i < (tile ? 1 : it.ntok) * Sh::kHalves; i += 32) {
           const int h = i % Sh::kHalves, tk = i / Sh::kHalves;
           tma_load_3d(smem_u32(smem) + h * Sh::kQHalf + tk * p.G * 128, tile ? &tmap_tile : &tmap_token, &sh->qfull,
@@ -638,13 +656,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         }
         return true;
       };
-      int pg0 = page_at(0), pg1 = page_at(1);  // of tiles j and j + 1
-      ok = load(false, 0, pg0) && load_q() && (n == 1 || load(false, 1, pg1));
-      for (int j = 0; ok && j < n; ++j) {
-        const int pg2 = page_at(j + 2);
-        ok = load(true, j, pg0) && (j + 2 >= n || load(false, j + 2, pg2));
+      // K0, Q, K1, V0, K2, V1, ...: in one loop, as the code of four calls took its time to fetch
+      int pg0 = 0, pg1 = 0, pg2 = page_at(0);  // of tiles t - 2, t - 1 and t
+#pragma unroll 1
+      for (int t = 0; ok && t < n + 2; ++t) {
+        const int pg3 = page_at(t + 1);
+        ok = (t < 2 || load(true, t - 2, pg0)) && (t >= n || load(false, t, pg2)) && (t != 0 || load_q());
         pg0 = pg1;
         pg1 = pg2;
+        pg2 = pg3;
       }
     }
   } else if (warp == 5) {
@@ -679,6 +699,25 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       advance();
       return true;
     };
+    auto values = [&](int b, int j, int n) {  // O += P V, P in buffer b, V at the current place
+      if (!wait_warp(&sh->full[st], ph, p.err, abort) || !wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort))
+        return false;
+      p_ph ^= 1u << b;
+      tc_fence_after();
+      if (elect_one()) {
+        uint32_t d = tmem_u + 2 * kKeys, a = tmem_u + b * kKeys, vd = ring_v + st * (Sh::kKvBytes >> 4);
+        opaque(d, a, vd);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          mma_ts<D>(d, a + kk * 8, vd + kk * (2 * Sh::kKvGroup >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(j != 0));
+        umma_commit(&sh->empty[st]);
+        if (j == n - 2) umma_commit(&sh->olast);
+        if (j == n - 1) umma_commit(&sh->ofull);
+      }
+      __syncwarp();
+      advance();
+      return true;
+    };
     bool ok = true;
     for (int k = 0; ok && next_item(k); ++k) {
       const Item& it = item_at(k);
@@ -686,26 +725,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (lane == 0) done(k);
       ok = wait_warp(&sh->qfull, q_ph, p.err, abort);
       q_ph ^= 1;
-      ok = ok && scores(0, n == 1) && (n == 1 || scores(1, n == 2));
-      for (int j = 0; ok && j < n; ++j) {  // O += P V of tile j, then the scores of tile j + 2
-        const int b = j & 1;
-        ok = wait_warp(&sh->full[st], ph, p.err, abort) && wait_warp(&sh->pfull[b], (p_ph >> b) & 1, p.err, abort);
-        if (!ok) break;
-        p_ph ^= 1u << b;
-        tc_fence_after();
-        if (elect_one()) {
-          uint32_t d = tmem_u + 2 * kKeys, a = tmem_u + b * kKeys, vd = ring_v + st * (Sh::kKvBytes >> 4);
-          opaque(d, a, vd);
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_ts<D>(d, a + kk * 8, vd + kk * (2 * Sh::kKvGroup >> 4), idesc_o, kk ? 1u : static_cast<uint32_t>(j != 0));
-          umma_commit(&sh->empty[st]);
-          if (j == n - 2) umma_commit(&sh->olast);
-          if (j == n - 1) umma_commit(&sh->ofull);
-        }
-        __syncwarp();
-        advance();
-        if (j + 2 < n) ok = scores(b, j + 3 == n);
+#pragma unroll 1
+      for (int t = 0; ok && t < n + 2; ++t) {  // O += P V of tile t - 2, then the scores of tile t
+        const int b = t & 1;
+        if (t >= 2) ok = values(b, t - 2, n);
+        if (ok && t < n) ok = scores(b, t == n - 1);
       }
     }
   } else {
@@ -733,7 +757,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const int r = tid >> 1, key = (x.lo + j) * kKeys + r;  // two threads a row
       if (key >= x.full) {
         const bool beyond = key >= x.need;
-#pragma unroll
+#pragma unroll 2
         for (int q = 0; q < D / 16; ++q) {
           const int c = q * 2 + (tid & 1);  // 16-byte chunk of the row
           uint4* at = reinterpret_cast<uint4*>(tile + (r >> 3) * Sh::kKvGroup + (c >> 3) * 1024 + (r & 7) * 128 + (((c + r) & 7) << 4));
@@ -882,7 +906,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (n > 1) last_ph ^= 1;  // (completed before ofull)
       tc_fence_after();
       if (busy) {
-        const bool bad = sh->bad[k & 1] == k + 1;
         const float norm = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const size_t out_row = static_cast<size_t>(it.first + my_token) * p.Hq + it.h * p.G + (row - rt * p.G);
         float* part = p.part + (static_cast<size_t>(place) * 2 + slot) * Sh::kPartFloats;
@@ -893,21 +916,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           tmem_ld_wait();
 #pragma unroll
           for (int q = 0; q < 32; ++q) o[q] *= norm;
-          if (bad && live) {  // values that were kept out of the MMA
-            for (int key = max(full, lo * kKeys); key < min(it.need, it.hi * kKeys); ++key) {
-              if (!(visible(p, it, my_token, key) & 1)) continue;
-              const int page = p.table[static_cast<long long>(it.b) * p.table_stride + (key >> p.page_shift)];
-              if (page < 0 || page >= p.num_pages) continue;
-              const uint16_t* v = p.v + page * p.cs.page + (key & ((1 << p.page_shift) - 1)) * p.cs.row +
-                                  it.h * p.cs.head + c;
-#pragma unroll
-              for (int q = 0; q < 32; ++q) {
-                const float e = BF16 ? __uint_as_float(static_cast<uint32_t>(v[q]) << 16)
-                                     : __half2float(__ushort_as_half(v[q]));
-                if (!isfinite(e)) o[q] += e;
-              }
-            }
-          }
           if (!live) continue;
           if (whole) {
             uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * D + c);
@@ -921,6 +929,27 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             float4* dst = reinterpret_cast<float4*>(part) + ((c / 4) << lg) + row;
 #pragma unroll
             for (int q = 0; q < 8; ++q) dst[q << lg] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          }
+        }
+        // Values that were kept out of the MMA: infinities and NaNs, so they may as well be
+        // added to what has been written.
+        if (sh->bad[k & 1] == k + 1 && live) {
+#pragma unroll 1
+          for (int key = max(full, lo * kKeys); key < min(it.need, it.hi * kKeys); ++key) {
+            const int page = p.table[static_cast<long long>(it.b) * p.table_stride + (key >> p.page_shift)];
+            if (page < 0 || page >= p.num_pages || !(visible(p, it, my_token, key) & 1)) continue;
+            const uint16_t* v = p.v + page * p.cs.page + (key & ((1 << p.page_shift) - 1)) * p.cs.row + it.h * p.cs.head;
+#pragma unroll 1
+            for (int c = 0; c < D; ++c) {
+              const float e = value<BF16>(v[c]);
+              if (isfinite(e)) continue;
+              uint16_t* o16 = p.out + out_row * D + c;
+              float* o32 = part + (((c >> 2) << log2_up(rows)) + row) * 4 + (c & 3);
+              if (whole)
+                *o16 = static_cast<uint16_t>(pack_pair<BF16>(value<BF16>(*o16) + e, 0.f));
+              else
+                *o32 += e;
+            }
           }
         }
         if (live) {
