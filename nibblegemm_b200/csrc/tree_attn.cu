@@ -656,15 +656,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         }
         return true;
       };
-      // K0, Q, K1, V0, K2, V1, ...: in one loop, as the code of four calls took its time to fetch
-      int pg0 = 0, pg1 = 0, pg2 = page_at(0);  // of tiles t - 2, t - 1 and t
-#pragma unroll 1
-      for (int t = 0; ok && t < n + 2; ++t) {
-        const int pg3 = page_at(t + 1);
-        ok = (t < 2 || load(true, t - 2, pg0)) && (t >= n || load(false, t, pg2)) && (t != 0 || load_q());
+      int pg0 = page_at(0), pg1 = page_at(1);  // of tiles j and j + 1
+      ok = load(false, 0, pg0) && load_q() && (n == 1 || load(false, 1, pg1));
+      for (int j = 0; ok && j < n; ++j) {
+        const int pg2 = page_at(j + 2);
+        ok = load(true, j, pg0) && (j + 2 >= n || load(false, j + 2, pg2));
         pg0 = pg1;
         pg1 = pg2;
-        pg2 = pg3;
       }
     }
   } else if (warp == 5) {
