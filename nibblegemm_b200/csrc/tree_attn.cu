@@ -49,8 +49,9 @@
 // 32 query heads, 8 KV heads of 128, bf16, on a B200:
 //   64 single tokens, up to 8192 rows   205 us  6.4 TB/s
 //   32 trees of up to 64, 4096 rows     102 us  3.5 TB/s, 625 TFLOP/s
-//   3 x up to 2048 tokens, 4096 rows    340 us  1035 TFLOP/s
-//   1 token, 777 rows (fp16)           11.5 us
+//   3 x up to 2048 tokens, 4096 rows    343 us  1025 TFLOP/s
+//   1000 single tokens, up to 500 rows  213 us  5.9 TB/s
+//   1 token, 777 rows (fp16)           10.8 us
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -1021,7 +1022,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
       const bool mine = row < mt.rows && e < end;
       Joined j{-INFINITY, 0.f, {}};
       if (mine) {
-#pragma unroll 4
+#pragma unroll 1  // (four at a time: more code to fetch, 0.3 us on a small call, and no less for 37 parts)
         for (int k = k0; k < mt.parts; k += step) {
           const float* src = p.part + (static_cast<size_t>(mt.first + k) * 2 + (k == 0)) * Shape<D>::kPartFloats;
           const float4* v = reinterpret_cast<const float4*>(src) + (chunk << (lg + 1)) + row;
