@@ -390,7 +390,7 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
  *     or NULL: the chain, j <= i) and sees all rows before them.  A row that sees
  *     nothing gives zeros.  lse [T, Hq] (may be NULL): log of the sum of
  *     exponentials, -inf for such a row.  D 64 or 128, Hq / Hkv <= 128, scale > 0.
- *     workspace: ng_tree_attn_workspace_bytes(D) bytes, 256-byte aligned; calls sharing it must
+ *     workspace: ng_tree_attn_workspace_bytes(D) bytes (79 MB for D 128), 256-byte aligned; calls sharing it must
  *     not overlap on the GPU.  A page outside the pool reads as zeros and sets
  *     NG_ERR_BAD_INDEX in ng_device_status.
  *   ng_tree_commit: greedy acceptance.  The path starts at node 0 and goes on to

@@ -392,10 +392,10 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
 
 // Bounded wait; false once the CTA has given up.  Plain polling measured fastest: a
 // suspend-time hint or a nanosleep between polls adds its wake-up to a chain of short
-// hand-overs (one token, 777 rows: 12.8 us as it is, 14 and more with either).
-// Kept short, as there are many of them: one place that polls, and the low word of the timer
-// (nanoseconds; it wraps after four seconds).  Reading it also paces the polls: with the
-// clock instead the waiting warps took issue slots from the others (chains 357 us, 340 so).
+// hand-overs (one token, 777 rows: 1.5 us more with either).  Kept short, as there are many
+// of them, with the low word of the timer (nanoseconds; it wraps after four seconds).  Reading
+// it also paces the polls: with the clock instead, the waiting warps took issue slots
+// from the others (chains 357 us instead of 343).
 __device__ __forceinline__ uint32_t timer_ns() {
   uint32_t t;
   asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
