@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <mutex>
 #include <optional>
 #include <tuple>
@@ -60,23 +61,34 @@ torch::Tensor output(const std::optional<torch::Tensor>& out, int64_t M, int64_t
   return o;
 }
 
-// Zero-filled workspace per (device, stream, kind), grown on demand.  Every
-// call leaves its counters at zero, so the buffer is reused as is; one per
-// stream because calls sharing a workspace must not overlap on the GPU.
+// Kinds of workspace.
+constexpr int kGemvWorkspace = 0, kGemmWorkspace = 1, kAttentionWorkspace = 2;
+
+// The cached workspace of (device, stream, kind), grown on demand; one per stream,
+// because calls sharing a workspace must not overlap on the GPU.  Those of the GEMV and the
+// GEMM are zero-filled, once: every call leaves their counters at zero.  The attention needs
+// no zeros, and its buffer has the size of its largest form from the start, so it never grows.
+//
+// A captured CUDA graph keeps the address, so a buffer that was outgrown is never freed (each is
+// at least twice the one before, so all of them are less than twice the last).
 torch::Tensor workspace(const torch::Device& dev, cudaStream_t stream, int kind, size_t need) {
   // Heap-held and never destroyed: a static map of tensors would be torn down at
   // process exit after torch's CUDA allocator, and crash there.
   static std::mutex mu;
-  static auto* cache = new std::unordered_map<uint64_t, torch::Tensor>();
+  static auto* cache = new std::unordered_map<uint64_t, std::vector<torch::Tensor>>();  // the last one is in use
   const uint64_t key = (reinterpret_cast<uint64_t>(stream) << 8) ^ (static_cast<uint64_t>(dev.index()) << 2) ^
                        static_cast<uint64_t>(kind);
   std::lock_guard<std::mutex> lock(mu);
-  auto it = cache->find(key);
-  if (it != cache->end() && static_cast<size_t>(it->second.numel()) >= need) return it->second;
-  const int64_t bytes = static_cast<int64_t>(std::max<size_t>(need, kind == 0 ? (4u << 20) : (1u << 20)));
-  auto ws = torch::zeros({bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
-  (*cache)[key] = ws;
-  return ws;
+  auto& all = (*cache)[key];
+  const size_t have = all.empty() ? 0 : static_cast<size_t>(all.back().numel());
+  if (have >= std::max<size_t>(need, 1)) return all.back();
+  const c10::cuda::CUDAGuard guard(dev);
+  const size_t least = kind == kAttentionWorkspace ? ng_tree_attn_workspace_bytes(128) : kind == kGemvWorkspace ? 4u << 20 : 1u << 20;
+  const auto bytes = static_cast<int64_t>(std::max({need, 2 * have, least}));
+  const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
+  auto make = [&] { return kind == kAttentionWorkspace ? torch::empty({bytes}, options) : torch::zeros({bytes}, options); };
+  all.push_back(make());
+  return all.back();
 }
 
 std::tuple<torch::Tensor, int64_t> gemv_w4a16(torch::Tensor X, torch::Tensor Wq, torch::Tensor S, int64_t group_size,
@@ -93,7 +105,7 @@ std::tuple<torch::Tensor, int64_t> gemv_w4a16(torch::Tensor X, torch::Tensor Wq,
   const c10::cuda::CUDAGuard guard(X.device());
   auto Y = output(out, M, N, X);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(X.device().index()).stream();
-  auto ws = workspace(X.device(), stream, 0, ng_gemv_workspace_bytes(1, static_cast<int>(N)));
+  auto ws = workspace(X.device(), stream, kGemvWorkspace, ng_gemv_workspace_bytes(1, static_cast<int>(N)));
   const int st = ng_gemv_w4a16(X.data_ptr(), dtype_code(X), Wq.data_ptr<int32_t>(),
                              reinterpret_cast<const uint16_t*>(S.data_ptr()), Y.data_ptr(),
                              static_cast<int>(M), static_cast<int>(K), static_cast<int>(N),
@@ -109,7 +121,7 @@ std::tuple<torch::Tensor, int64_t> gemm_w4a16(torch::Tensor X, torch::Tensor Wq,
   const c10::cuda::CUDAGuard guard(X.device());
   auto Y = output(out, M, N, X);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(X.device().index()).stream();
-  auto ws = workspace(X.device(), stream, 1, ng_gemm_workspace_bytes(static_cast<int>(M), static_cast<int>(N)));
+  auto ws = workspace(X.device(), stream, kGemmWorkspace, ng_gemm_workspace_bytes(static_cast<int>(M), static_cast<int>(N)));
   const int st = ng_gemm_w4a16(X.data_ptr(), dtype_code(X), Wq.data_ptr<int32_t>(),
                              reinterpret_cast<const uint16_t*>(S.data_ptr()), Y.data_ptr(),
                              static_cast<int>(M), static_cast<int>(K), static_cast<int>(N),
@@ -302,7 +314,7 @@ std::tuple<torch::Tensor, std::optional<torch::Tensor>, int64_t> tree_attention(
   if (return_lse) lse = torch::empty({T, Hq}, q.options().dtype(torch::kFloat));
   if (T == 0 || B == 0) return {y, lse, 0};
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  auto ws = workspace(dev, stream, 2, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
+  auto ws = workspace(dev, stream, kAttentionWorkspace, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
   const int st = ng_tree_attn(
       q.data_ptr(), q.stride(0), q.stride(1), K.data_ptr(), V.data_ptr(), K.stride(0), K.stride(1), K.stride(2),
       table.data_ptr<int>(), stride, static_cast<int>(table.size(1)), kv_lens.data_ptr<int>(),
@@ -372,7 +384,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_w4a16", &gemm_w4a16, "Prefill-regime W4A16 GEMM (tcgen05).", py::arg("X"), py::arg("Wq"),
         py::arg("S"), py::arg("group_size"), py::arg("version") = 6, py::arg("tile_tokens") = 0,
         py::arg("out") = py::none());
-  m.def("workspace", &workspace_for, "The zero-initialised workspace of (device, stream); kind 0 = GEMV, 1 = GEMM, 2 = tree attention.",
+  m.def("workspace", &workspace_for, "The cached workspace of (device, stream); kind 0 = GEMV, 1 = GEMM (both zero-initialised), 2 = tree attention.",
         py::arg("device_index"), py::arg("stream"), py::arg("kind"), py::arg("need"));
   m.def("paged_plan", &paged_plan);
   m.def("qk_norm_rope_append", &qk_norm_rope_append);

@@ -126,6 +126,7 @@ class _Extension:
         self.binding = _load_binding()
         self._ws = {}  # (device index, stream handle) -> zero-initialised GEMV workspace
         self._gws = {}  # (device index, stream handle) -> zero-initialised GEMM split-K workspace
+        self._outgrown = []  # earlier ones: a captured graph may hold their addresses
 
     def gemm_workspace(self, M: int, N: int, device: torch.device, stream: int) -> torch.Tensor:
         """The prefill-GEMM split-K workspace for (device, stream), grown on demand
@@ -136,7 +137,11 @@ class _Extension:
         key = (device.index, stream)
         ws = self._gws.get(key)
         if ws is None or ws.numel() < need:
-            ws = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
+            have = 0
+            if ws is not None:
+                self._outgrown.append(ws)
+                have = ws.numel()
+            ws = torch.zeros(max(need, 2 * have, 1 << 20), dtype=torch.uint8, device=device)
             self._gws[key] = ws
         return ws
 
@@ -153,7 +158,11 @@ class _Extension:
         key = (device.index, stream)
         ws = self._ws.get(key)
         if ws is None or ws.numel() < need:
-            ws = torch.zeros(max(need, 4 << 20), dtype=torch.uint8, device=device)
+            have = 0
+            if ws is not None:
+                self._outgrown.append(ws)
+                have = ws.numel()
+            ws = torch.zeros(max(need, 2 * have, 4 << 20), dtype=torch.uint8, device=device)
             self._ws[key] = ws
         return ws
 

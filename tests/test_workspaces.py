@@ -1,0 +1,79 @@
+"""The cached scratch memory of the compiled binding, beside CUDA graphs that hold its
+addresses: it never moves under a graph."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import nibblegemm_b200 as ng
+from tests import test_paged as tp
+
+pytestmark = pytest.mark.gpu
+
+GEMV, GEMM, ATTENTION = 0, 1, 2
+
+
+def fresh_stream():
+    """A stream that no call has used (torch.cuda.Stream() hands out 32 of them in turn)."""
+    handle = ctypes.c_void_p()
+    assert int(torch.cuda.cudart().cudaStreamCreate(ctypes.addressof(handle))) == 0
+    return torch.cuda.ExternalStream(handle.value)
+
+
+def scratch(stream, kind, need=0):
+    return ng.extension().binding.workspace(torch.cuda.current_device(), stream.cuda_stream, kind, need)
+
+
+def attention_inputs(dim, new, kv, hq=8, hk=2, dtype=torch.float16, seed=0):
+    rng = np.random.default_rng(seed)
+    torch.manual_seed(seed)
+    k, v, table = tp.build_pages(rng, kv, 16, hk, dim, dtype, False)
+    q = torch.randn(sum(new), hq, dim, device="cuda").to(dtype)
+    return q, k, v, table, tp.ints(kv), tp.ints(np.concatenate([[0], np.cumsum(new)]))
+
+
+def test_attention_scratch_does_not_move():
+    s = fresh_stream()
+    with torch.cuda.stream(s):
+        ng.tree_attention(*attention_inputs(64, [3], [500]))
+        first = scratch(s, ATTENTION).data_ptr()
+        ng.tree_attention(*attention_inputs(128, [3], [500]))
+        assert scratch(s, ATTENTION).data_ptr() == first
+    tp.assert_clean()
+
+
+@pytest.mark.parametrize("kind", [GEMV, GEMM])
+def test_an_outgrown_buffer_stays_allocated(kind):
+    """A graph captured before the buffer grew still writes to the old one."""
+    s = fresh_stream()
+    with torch.cuda.stream(s):
+        w = scratch(s, kind, 1)
+        old, size = w.data_ptr(), w.numel()
+        del w
+        assert scratch(s, kind, size + 1).data_ptr() != old
+        others = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        assert all(not old <= x.data_ptr() < old + size for x in others)
+        assert not scratch(s, kind).any()
+
+
+def test_a_captured_call_beside_later_calls():
+    """A graph of a small head size, then calls of a large one on its stream: replays write nothing
+    that is not theirs."""
+    small, large = attention_inputs(64, [3, 40], [5000, 300]), attention_inputs(128, [3, 40], [5000, 300])
+    want = ng.tree_attention(*small)
+    torch.cuda.synchronize()
+    s, graph, out = fresh_stream(), torch.cuda.CUDAGraph(), torch.empty_like(want)
+    with torch.cuda.stream(s):
+        ng.tree_attention(*small)
+        with torch.cuda.graph(graph, stream=s):
+            ng.tree_attention(*small, out=out)
+        ng.tree_attention(*large)
+        others = [torch.full((n << 20,), 5, dtype=torch.uint8, device="cuda") for n in (1, 4, 20, 40, 45, 80)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert all((x == 5).all() for x in others)
+    tp.assert_clean()
