@@ -8,6 +8,7 @@
 // reference's do; the library's own status is returned beside the output and
 // the Python wrapper raises on a non-zero one.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -69,8 +70,12 @@ constexpr int kGemvWorkspace = 0, kGemmWorkspace = 1, kAttentionWorkspace = 2;
 // GEMM are zero-filled, once: every call leaves their counters at zero.  The attention needs
 // no zeros, and its buffer has the size of its largest form from the start, so it never grows.
 //
-// A captured CUDA graph keeps the address, so a buffer that was outgrown is never freed (each is
-// at least twice the one before, so all of them are less than twice the last).
+// A captured CUDA graph keeps the address, so
+// * a buffer that was outgrown is never freed (each is at least twice the one before, so all
+//   of them are less than twice the last);
+// * no buffer is made by a capture, whose graph would own it and fill it with zeros again at
+//   every replay (and at the replay only): one that is first asked for during a capture is made
+//   beside it, on a stream that is not captured.
 torch::Tensor workspace(const torch::Device& dev, cudaStream_t stream, int kind, size_t need) {
   // Heap-held and never destroyed: a static map of tensors would be torn down at
   // process exit after torch's CUDA allocator, and crash there.
@@ -87,7 +92,23 @@ torch::Tensor workspace(const torch::Device& dev, cudaStream_t stream, int kind,
   const auto bytes = static_cast<int64_t>(std::max({need, 2 * have, least}));
   const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
   auto make = [&] { return kind == kAttentionWorkspace ? torch::empty({bytes}, options) : torch::zeros({bytes}, options); };
-  all.push_back(make());
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
+    all.push_back(make());
+  } else {
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    auto beside = c10::cuda::getStreamFromPool(false, dev.index());
+    auto captured = [&] {
+      const c10::cuda::CUDAStreamGuard on(beside);
+      return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+    };
+    for (int i = 0; i < 32 && captured(); ++i) beside = c10::cuda::getStreamFromPool(false, dev.index());  // it has 32
+    TORCH_CHECK(!captured(), "no stream is left to make a workspace on beside the capture");
+    {
+      const c10::cuda::CUDAStreamGuard on(beside);
+      all.push_back(make());
+    }
+    beside.synchronize();
+  }
   return all.back();
 }
 

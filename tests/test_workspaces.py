@@ -1,5 +1,5 @@
 """The cached scratch memory of the compiled binding, beside CUDA graphs that hold its
-addresses: it never moves under a graph."""
+addresses: it never moves under a graph, and no graph owns it."""
 from __future__ import annotations
 
 import ctypes
@@ -25,6 +25,14 @@ def fresh_stream():
 
 def scratch(stream, kind, need=0):
     return ng.extension().binding.workspace(torch.cuda.current_device(), stream.cuda_stream, kind, need)
+
+
+def pool_of(pointer):
+    """Which of the allocator's pools an address lies in; (0, 0) is the one that no graph owns."""
+    for s in torch.cuda.memory_snapshot():
+        if s["address"] <= pointer < s["address"] + s["total_size"]:
+            return tuple(s["segment_pool_id"])
+    return None
 
 
 def attention_inputs(dim, new, kv, hq=8, hk=2, dtype=torch.float16, seed=0):
@@ -57,6 +65,34 @@ def test_an_outgrown_buffer_stays_allocated(kind):
         others = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
         assert all(not old <= x.data_ptr() < old + size for x in others)
         assert not scratch(s, kind).any()
+
+
+def test_first_call_in_a_capture():
+    """The capture owns no buffer that later calls use, and those are zero before its first replay."""
+    torch.manual_seed(0)
+    K, N = 512, 1024
+    qw = ng.quantize(torch.randn(K, N)).to("cuda")
+    x, many = (torch.randn(m, K, device="cuda").half() for m in (1, 128))
+    inputs = attention_inputs(64, [3], [500])
+    calls = (lambda: ng.gemv(x, qw)), (lambda: ng.gemm(many, qw)), (lambda: ng.tree_attention(*inputs))
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    s, graph = fresh_stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = [f() for f in calls]
+    with torch.cuda.stream(s):
+        for kind in (GEMV, GEMM, ATTENTION):
+            assert pool_of(scratch(s, kind, 1).data_ptr()) == (0, 0)
+        for kind in (GEMV, GEMM):
+            assert not scratch(s, kind).any()
+        again = [f() for f in calls]  # before any replay
+        for y, w in zip(again, want):
+            assert torch.equal(y, w)
+        graph.replay()
+    torch.cuda.synchronize()
+    for y, w in zip(got, want):
+        assert torch.equal(y, w)
+    tp.assert_clean()
 
 
 def test_a_captured_call_beside_later_calls():
