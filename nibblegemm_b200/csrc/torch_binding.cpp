@@ -112,6 +112,14 @@ torch::Tensor workspace(const torch::Device& dev, cudaStream_t stream, int kind,
   return all.back();
 }
 
+// The attention's workspace for one call.  In a capture it comes from the graph's own
+// memory: graphs captured on one stream may be replayed at the same time.
+torch::Tensor attention_workspace(const torch::Device& dev, cudaStream_t stream, size_t need) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+    return workspace(dev, stream, kAttentionWorkspace, need);
+  return torch::empty({static_cast<int64_t>(need)}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+}
+
 std::tuple<torch::Tensor, int64_t> gemv_w4a16(torch::Tensor X, torch::Tensor Wq, torch::Tensor S, int64_t group_size,
                          int64_t version, int64_t splits_override, int64_t threads_override,
                          int64_t algo, std::optional<torch::Tensor> out) {
@@ -335,7 +343,7 @@ std::tuple<torch::Tensor, std::optional<torch::Tensor>, int64_t> tree_attention(
   if (return_lse) lse = torch::empty({T, Hq}, q.options().dtype(torch::kFloat));
   if (T == 0 || B == 0) return {y, lse, 0};
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-  auto ws = workspace(dev, stream, kAttentionWorkspace, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
+  auto ws = attention_workspace(dev, stream, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
   const int st = ng_tree_attn(
       q.data_ptr(), q.stride(0), q.stride(1), K.data_ptr(), V.data_ptr(), K.stride(0), K.stride(1), K.stride(2),
       table.data_ptr<int>(), stride, static_cast<int>(table.size(1)), kv_lens.data_ptr<int>(),

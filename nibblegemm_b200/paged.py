@@ -143,7 +143,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     chains, prompts and single tokens need none.  A token that sees nothing gives
     zeros.  ``scale`` defaults to 1 / sqrt(D).  Returns out like q, and with
     ``return_lse`` also the fp32 [tokens, q_heads] logarithm of the sum of
-    exponentials (-inf where nothing is seen).  D 64 or 128."""
+    exponentials (-inf where nothing is seen).  D 64 or 128.
+
+    Scratch memory (79 MB) is kept for each stream; a call that is captured takes it from its
+    graph's own memory, so graphs may be replayed at the same time."""
     y, lse, status = _binding().tree_attention(q, k_cache, v_cache, block_table, kv_lens, cu_new, mask,
                                                q.size(-1) ** -0.5 if scale is None else scale, return_lse, out)
     _done(status, "tree_attention")

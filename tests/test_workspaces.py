@@ -1,5 +1,6 @@
 """The cached scratch memory of the compiled binding, beside CUDA graphs that hold its
-addresses: it never moves under a graph, and no graph owns it."""
+addresses: it never moves under a graph, no graph owns it, and two graphs captured on
+one stream may run at the same time."""
 from __future__ import annotations
 
 import ctypes
@@ -112,4 +113,30 @@ def test_a_captured_call_beside_later_calls():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         assert all((x == 5).all() for x in others)
+    tp.assert_clean()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_graphs_of_one_stream_replayed_at_the_same_time(dim):
+    """torch.cuda.graph captures on one stream unless it is told otherwise.  (Several parts an item,
+    so that the scratch memory is used.)"""
+    inputs = [attention_inputs(dim, new, kv, seed=i) for i, (new, kv) in enumerate((([3, 40], [9000, 3000]), ([16], [14000])))]
+    want = [ng.tree_attention(*x) for x in inputs]
+    torch.cuda.synchronize()
+    outs, graphs = [torch.empty_like(w) for w in want], [torch.cuda.CUDAGraph() for _ in want]
+    for x, out, graph in zip(inputs, outs, graphs):
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                ng.tree_attention(*x, out=out)
+    streams = [torch.cuda.Stream() for _ in want]
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
     tp.assert_clean()
