@@ -364,7 +364,7 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
  *   ng_paged_plan: the plan of a step from the requests' lengths, in order:
  *     need[b] = max(0, ceil((cached[b] + new[b]) / page_size) - held[b]) pages, taken from
  *     free_pages[cursor ..] (cursor: device int or NULL = 0).  A request whose
- *     pages are not there, or do not fit its table row, is not granted: its
+ *     pages are not there, or do not fit its table row (it needs none then), is not granted: its
  *     slots are -1, its kv_lens 0, its table row and held_out as before.
  *     Outputs: cu_new [B + 1]; per token slots (page * page_size + row),
  *     positions (cached + depth in its tree; + its place without parents), mask

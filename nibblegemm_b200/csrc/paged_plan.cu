@@ -1,9 +1,10 @@
 // Plan of one step over a paged KV cache, built on the GPU from the requests'
 // lengths, so that a serving loop (or a CUDA graph of it) never reads them back:
-//   need[b]   = max(0, ceil((cached[b] + new[b]) / page) - held[b])   pages to take
+//   blocks[b] = ceil((cached[b] + new[b]) / page)
+//   need[b]   = max(0, blocks[b] - held[b]) pages to take; 0 if the blocks do not fit the
+//               table's row: such a request gets nothing, and its pages are left to the others
 //   off       = exclusive prefix sum of need over the requests, in order
-//   granted b : need[b] == 0, or off[b] + need[b] <= free pages left; and the
-//               blocks fit the table's row
+//   granted b : the blocks fit, and need[b] == 0 or off[b] + need[b] <= free pages left
 //   table[b, held[b] + i] = free[cursor + off[b] + i]
 //   slot(b, i) = table[b, (cached + i) / page] * page + (cached + i) % page
 //   position(b, i) = cached[b] + depth of node i (no tree: + i)
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   const int used = p.cursor ? min(max(*p.cursor, 0), p.num_free) : 0;
   const int available = p.num_free - used;
 
-  auto lengths = [&](int b, int& cached, int& fresh, int& held, int& blocks) {
+  auto lengths = [&](int b, int& cached, int& fresh, int& held, int& blocks, int& need) {
     cached = p.cached[b];
     fresh = p.new_lens[b];
     held = p.held[b];
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
       held = max(held, 0);
     }
     blocks = (cached + fresh + ps - 1) >> p.page_shift;
+    need = blocks <= p.table_width ? max(0, blocks - held) : 0;
   };
 
   // ---- both prefix sums: a contiguous run of requests per thread
@@ -98,10 +100,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   const int b0 = min(B, tid * per), b1 = min(B, b0 + per);
   Pair mine = {0, 0};
   for (int b = b0; b < b1; ++b) {
-    int cached, fresh, held, blocks;
-    lengths(b, cached, fresh, held, blocks);
+    int cached, fresh, held, blocks, need;
+    lengths(b, cached, fresh, held, blocks, need);
     mine.a += fresh;
-    mine.b += max(0, blocks - held);
+    mine.b += need;
   }
   Pair inc = mine;
   for (int o = 1; o < 32; o <<= 1) {
@@ -125,9 +127,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   // that still reads as "beyond the end".
   auto clip = [](long long v, long long top) { return static_cast<int>(v < top ? v : top); };
   for (int b = b0; b < b1; ++b) {
-    int cached, fresh, held, blocks;
-    lengths(b, cached, fresh, held, blocks);
-    const int need = max(0, blocks - held);
+    int cached, fresh, held, blocks, need;
+    lengths(b, cached, fresh, held, blocks, need);
     cu[b] = clip(run.a, p.tokens);
     ends[b] = clip(run.b, 0x7fffffff);
     const bool granted = (need == 0 || run.b + need <= available) && blocks <= p.table_width;
@@ -157,10 +158,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   const int fresh_pages = min(ends[B], available);
   for (int j = start; j < fresh_pages; j += stride) {
     const int b = find_request(ends, B, j);
-    int cached, fresh, held, blocks;
-    lengths(b, cached, fresh, held, blocks);
-    const int need = max(0, blocks - held);
-    if (ends[b] + need > available || blocks > p.table_width) continue;  // not granted
+    int cached, fresh, held, blocks, need;
+    lengths(b, cached, fresh, held, blocks, need);
+    if (ends[b] + need > available) continue;  // not granted
     const int col = held + j - ends[b];
     p.table[static_cast<size_t>(b) * p.table_stride + col] = p.free_pages[used + j];
   }
@@ -175,9 +175,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     }
     const int b = find_request(cu, B, t);
     const int i = t - cu[b];
-    int cached, fresh, held, blocks;
-    lengths(b, cached, fresh, held, blocks);
-    const int need = max(0, blocks - held);
+    int cached, fresh, held, blocks, need;
+    lengths(b, cached, fresh, held, blocks, need);
     const bool granted =
         (need == 0 || static_cast<long long>(ends[b]) + need <= available) && blocks <= p.table_width;
     int slot = -1;

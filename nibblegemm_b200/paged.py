@@ -98,7 +98,8 @@ def paged_plan(cached: torch.Tensor, new: torch.Tensor, held: torch.Tensor, bloc
     Pages are taken in request order from ``free_pages`` (int32), from entry
     ``cursor`` (int32 [1], default 0) on, and written into ``block_table``
     (int32 [requests, blocks], in place).  A request whose pages are not there or
-    do not fit its row of the table is not granted: slots -1, ``kv_lens`` 0.
+    do not fit its row of the table is not granted: slots -1, ``kv_lens`` 0.  One that
+    does not fit takes nothing from the others; ``taken`` counts the pages that were given out.
 
     ``num_tokens`` is the capacity of the per-token outputs (rows past the last
     new token get slot -1).  ``parents`` (int32 [num_tokens], within the request,

@@ -1,0 +1,61 @@
+"""Edges of the paged operators: requests that outgrow their row of the table."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import nibblegemm_b200 as ng
+from tests import test_paged as tp
+from tests.test_paged import ints
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------- plan
+def planned(cached, new, held, width, free, page):
+    """What each request gets: a request that does not fit its row of the table, or whose
+    pages are not there, gets nothing; only the others' pages count."""
+    off, kv, held_out, fresh = 0, [], [], []
+    for c, n, h in zip(cached, new, held):
+        blocks = -(-(c + n) // page)
+        need = max(0, blocks - h) if blocks <= width else 0
+        granted = blocks <= width and (need == 0 or off + need <= len(free))
+        fresh.append(free[off:off + need] if granted else [])
+        kv.append(c + n if granted else 0)
+        held_out.append(max(h, blocks) if granted else h)
+        off += need
+    return kv, held_out, fresh
+
+
+@pytest.mark.parametrize("B,width,short", [(3, 2, 0), (40, 5, 0), (40, 5, 6), (700, 9, 0), (700, 9, 200)])
+def test_plan_of_requests_that_outgrow_the_table(B, width, short):
+    rng = np.random.default_rng(B + short)
+    page = 16
+    cached = rng.integers(0, width * page + 1, B)
+    new = rng.integers(0, 2 * page, B)  # some end beyond their row
+    cached[0], new[0] = width * page, 1  # the first one among them
+    new[1:] = np.where(rng.random(B - 1) < 0.5, np.minimum(new[1:], width * page - cached[1:]), new[1:])
+    held = -(-cached // page)
+    blocks = -(-(cached + new) // page)
+    assert (blocks > width).any() and (blocks[1:] > held[1:]).any()
+    need = int(np.where(blocks <= width, np.maximum(blocks - held, 0), 0).sum())
+    pool = rng.permutation(int(held.sum()) + need + 20).tolist()
+    table = np.full((B, width), -1, np.int64)
+    for b in range(B):
+        table[b, :held[b]] = [pool.pop() for _ in range(held[b])]
+    free = pool[:need - short]  # exactly the pages that are needed, or too few
+    kv, held_out, fresh = planned(cached, new, held, width, free, page)
+    tab = ints(table)
+    p = ng.paged_plan(ints(cached), ints(new), ints(held), tab, ints(free), page_size=page, num_tokens=int(new.sum()))
+    for b in range(B):
+        table[b, held[b]:held[b] + len(fresh[b])] = fresh[b]
+    assert tab.tolist() == table.tolist()
+    assert p.kv_lens.tolist() == kv and p.held.tolist() == list(map(int, held_out))
+    assert p.taken.item() == sum(map(len, fresh))  # no page is counted that nobody has
+    slots, cu = p.slots.cpu().numpy(), p.cu_new.tolist()
+    for b in range(B):
+        at = cached[b] + np.arange(new[b])
+        want = table[b, np.minimum(at // page, width - 1)] * page + at % page if kv[b] else np.full(new[b], -1)
+        assert slots[cu[b]:cu[b + 1]].tolist() == want.tolist()
+    tp.assert_clean()
