@@ -374,7 +374,7 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
  *     NULL): index of the parent within the request, below the token's own, or
  *     -1.  num_tokens is the capacity of the per-token outputs; rows past the
  *     last token get slot -1, position 0, mask 0.  B <= 16384, mask_words <= 64.
- *     Negative lengths, more tokens than num_tokens, a parent that is not below
+ *     Lengths below 0 or from 2^30 on, more tokens than num_tokens, a parent that is not below
  *     its child, a tree beyond 64 * mask_words nodes: NG_ERR_BAD_INDEX in
  *     ng_device_status, and nothing is written out of bounds.
  *   ng_qk_norm_rope_append: rows of qkv [M, (Hq + 2 Hkv) * D] (row stride

@@ -27,6 +27,7 @@ namespace ngb {
 namespace {
 
 constexpr int kPlanThreads = 256;
+constexpr int kPlanMostTokens = (1 << 30) - 1;  // cached or new, of a request: their sum is an int
 constexpr int kPlanMaxBatch = 16384;  // two int prefix sums per request: 128 KB of shared memory
 
 struct PlanArgs {
@@ -85,13 +86,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     cached = p.cached[b];
     fresh = p.new_lens[b];
     held = p.held[b];
-    if (cached < 0 || fresh < 0 || held < 0 || cached > (1 << 30) || fresh > (1 << 30)) {
+    if (cached < 0 || fresh < 0 || held < 0 || cached > kPlanMostTokens || fresh > kPlanMostTokens) {
       atomicOr(p.err, kErrBadIndex);
-      cached = min(max(cached, 0), 1 << 30);
-      fresh = min(max(fresh, 0), 1 << 30);
+      cached = min(max(cached, 0), kPlanMostTokens);
+      fresh = min(max(fresh, 0), kPlanMostTokens);
       held = max(held, 0);
     }
-    blocks = (cached + fresh + ps - 1) >> p.page_shift;
+    // (rounded up without a sign: the sum may lie less than a page below 2^31)
+    blocks = static_cast<int>((static_cast<unsigned>(cached + fresh) + ps - 1) >> p.page_shift);
     need = blocks <= p.table_width ? max(0, blocks - held) : 0;
   };
 

@@ -1,4 +1,5 @@
-"""Edges of the paged operators: requests that outgrow their row of the table."""
+"""Edges of the paged operators: requests that outgrow their row of the table, and the
+largest lengths."""
 from __future__ import annotations
 
 import numpy as np
@@ -59,3 +60,17 @@ def test_plan_of_requests_that_outgrow_the_table(B, width, short):
         want = table[b, np.minimum(at // page, width - 1)] * page + at % page if kv[b] else np.full(new[b], -1)
         assert slots[cu[b]:cu[b + 1]].tolist() == want.tolist()
     tp.assert_clean()
+
+
+@pytest.mark.parametrize("cached,new", [(2**30, 2**30), (2**30 - 1, 2**30 - 1), (2**30 - 1, 4), (5, 2**30), (2**31 - 1, 8)])
+@pytest.mark.parametrize("page", [8, 1024])
+def test_plan_of_the_largest_lengths(cached, new, page):
+    """Lengths that no table holds are refused, not wrapped around to small ones."""
+    tab = ints([[0, -1, -1], [1, -1, -1]])
+    before = tab.clone()
+    p = ng.paged_plan(ints([3, cached]), ints([2, new]), ints([1, 1]), tab, ints([4, 5, 6]), page_size=page, num_tokens=10)
+    assert p.kv_lens.tolist() == [5, 0] and p.held.tolist() == [1, 1] and p.taken.item() == 0
+    assert p.slots.tolist() == [3, 4] + [-1] * 8
+    assert torch.equal(tab, before)
+    over = cached >= 2**30 or new >= 2**30 or new > 8  # the last: more tokens than there is room for
+    assert ng.extension().device_status() == (10 if over else 0)
