@@ -13,6 +13,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <limits>
 #include <mutex>
 #include <optional>
 #include <tuple>
@@ -341,7 +342,12 @@ std::tuple<torch::Tensor, std::optional<torch::Tensor>, int64_t> tree_attention(
   auto y = out.has_value() ? *out : torch::empty({T, Hq, D}, q.options());
   std::optional<torch::Tensor> lse;
   if (return_lse) lse = torch::empty({T, Hq}, q.options().dtype(torch::kFloat));
-  if (T == 0 || B == 0) return {y, lse, 0};
+  if (T == 0) return {y, lse, 0};
+  if (B == 0) {  // tokens of no request see nothing
+    y.zero_();
+    if (lse) lse->fill_(-std::numeric_limits<float>::infinity());
+    return {y, lse, 0};
+  }
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   auto ws = attention_workspace(dev, stream, ng_tree_attn_workspace_bytes(static_cast<int>(D)));
   const int st = ng_tree_attn(

@@ -141,8 +141,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``q`` [tokens, q_heads, D] may be strided.  A token sees every row before the
     new ones, and of those the ones its ``mask`` row names (int64 [tokens, words],
     bit j = new token j of the request); without a mask new token i sees 0 .. i, so
-    chains, prompts and single tokens need none.  A token that sees nothing gives
-    zeros.  ``scale`` defaults to 1 / sqrt(D).  Returns out like q, and with
+    chains, prompts and single tokens need none.  A token that sees nothing, or is no
+    request's, gives zeros.  ``scale`` defaults to 1 / sqrt(D).  Returns out like q, and with
     ``return_lse`` also the fp32 [tokens, q_heads] logarithm of the sum of
     exponentials (-inf where nothing is seen).  D 64 or 128.
 

@@ -1,5 +1,5 @@
-"""Edges of the paged operators: requests that outgrow their row of the table, and the
-largest lengths."""
+"""Edges of the paged operators: requests that outgrow their row of the table, the
+largest lengths, and tokens of no request."""
 from __future__ import annotations
 
 import numpy as np
@@ -74,3 +74,17 @@ def test_plan_of_the_largest_lengths(cached, new, page):
     assert torch.equal(tab, before)
     over = cached >= 2**30 or new >= 2**30 or new > 8  # the last: more tokens than there is room for
     assert ng.extension().device_status() == (10 if over else 0)
+
+
+# --------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_without_requests(dim):
+    """Tokens of no request give zeros, also when there are no requests at all."""
+    k, v = ng.paged_cache(2, 16, 2, dim)
+    q = torch.randn(5, 4, dim, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    got, lse = ng.tree_attention(q, k, v, torch.zeros(0, 3, dtype=torch.int32, device="cuda"), ints([]), ints([0]),
+                                 return_lse=True, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert (got == 0).all() and (lse == -float("inf")).all()
+    tp.assert_clean()
