@@ -388,7 +388,7 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
  *     request's first kv_lens[b] cache rows.  The last n = cu_new[b+1] - cu_new[b] of them are
  *     the new tokens' own: row i sees them by its mask bits (mask [T, mask_words]
  *     or NULL: the chain, j <= i) and sees all rows before them.  A row that sees
- *     nothing gives zeros.  lse [T, Hq] (may be NULL): log of the sum of
+ *     nothing, or lies in no request's range, gives zeros.  lse [T, Hq] (may be NULL): log of the sum of
  *     exponentials, -inf for such a row.  D 64 or 128, Hq / Hkv <= 128, scale > 0.
  *     workspace: ng_tree_attn_workspace_bytes(D) bytes (79 MB for D 128), 256-byte aligned; calls sharing it must
  *     not overlap on the GPU.  A page outside the pool reads as zeros and sets

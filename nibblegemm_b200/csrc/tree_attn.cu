@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   // ---- this CTA's shares of the lines
   const int per = (p.B + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-  const int tokens = min(max(p.cu[p.B], 0), p.T);
+  const int head = min(max(p.cu[0], 0), p.T), tokens = min(max(p.cu[p.B], head), p.T);
   long long mine[2] = {0, 0};
   Request req = {0, 0, 0, 0};
 #pragma unroll 1
@@ -565,13 +565,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     }
   }
   __syncthreads();
-  // rows beyond the last request's tokens see nothing
+  // rows in front of the first request's tokens and beyond the last one's see nothing
+  const long long row_chunks = static_cast<long long>(p.Hq) * (D / 8), gap = (tokens - head) * row_chunks;
 #pragma unroll 1
-  for (long long i = static_cast<long long>(tokens) * p.Hq * (D / 8) +
-                     static_cast<long long>(blockIdx.x) * kAttnThreads + tid;
-       i < static_cast<long long>(p.T) * p.Hq * (D / 8); i += static_cast<long long>(gridDim.x) * kAttnThreads) {
-    reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
-    if (p.lse && i % (D / 8) == 0) p.lse[i / (D / 8)] = -INFINITY;
+  for (long long i = static_cast<long long>(blockIdx.x) * kAttnThreads + tid; i < p.T * row_chunks - gap;
+       i += static_cast<long long>(gridDim.x) * kAttnThreads) {
+    const long long at = i < head * row_chunks ? i : i + gap;
+    reinterpret_cast<uint4*>(p.out)[at] = make_uint4(0, 0, 0, 0);
+    if (p.lse && at % (D / 8) == 0) p.lse[at / (D / 8)] = -INFINITY;
   }
   const uint32_t tmem = sh->tmem;
 

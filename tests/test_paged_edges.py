@@ -88,3 +88,20 @@ def test_attention_without_requests(dim):
     assert got.data_ptr() == out.data_ptr()
     assert (got == 0).all() and (lse == -float("inf")).all()
     tp.assert_clean()
+
+
+@pytest.mark.parametrize("first", [1, 40, 500])
+@pytest.mark.parametrize("end", [0, 3])
+def test_attention_rows_in_front_of_the_first_request(first, end):
+    rng = np.random.default_rng(0)
+    k, v, table = tp.build_pages(rng, [50, 20], 16, 2, 128, torch.float16, False)
+    T = first + 9 + end
+    q = torch.randn(T, 4, 128, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    cu = [first, first + 4, first + 9]
+    got, lse = ng.tree_attention(q, k, v, table, ints([50, 20]), ints(cu), return_lse=True, out=out)
+    assert (got[:first] == 0).all() and (lse[:first] == -float("inf")).all()
+    assert (got[cu[2]:] == 0).all() and (lse[cu[2]:] == -float("inf")).all()
+    want = ng.tree_attention(q[first:cu[2]], k, v, table, ints([50, 20]), ints([0, 4, 9]))
+    assert torch.equal(got[first:cu[2]], want)
+    tp.assert_clean()
