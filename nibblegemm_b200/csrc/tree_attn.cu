@@ -33,8 +33,8 @@
 // with their maxima and sums, which a second small kernel joins in a fixed order.
 //
 // The running maximum is only raised (and O rescaled) when it grows by more than
-// 8 in base 2: the probabilities then stay below 2^8, the sums are fp32, and
-// nearly all tiles leave O alone.  S, maxima, sums and O are fp32; P is
+// 8 in base 2: the probabilities then stay below 2^8 (fp16 keeps them 2^7 times as large,
+// see kLift), the sums are fp32, and nearly all tiles leave O alone.  S, maxima, sums and O are fp32; P is
 // rounded to the activation type, as the tensor core takes no other operand.
 //
 // Masked keys contribute nothing, whatever they hold: masked scores are replaced,
@@ -68,6 +68,12 @@ constexpr int kTile = 128;         // rows of a query tile
 constexpr int kKeys = 64;          // keys of a key tile
 constexpr int kAttnThreads = 192;  // 6 warps; two CTAs an SM leave 168 registers a thread
 constexpr float kRaise = 8.f;      // growth of the maximum (base 2) that is tolerated
+// Probabilities are kept times 2^kLift: fp16 ends at 2^16, which leaves 2^15 for those that
+// kRaise lets grow, and at its lower end loses what lies below 2^-25: 2^-32 of the running
+// maximum so, and 2^-25 of it without (131,000 keys just below that would be 0.4 % of a row).  bf16
+// has the exponents of fp32.
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.f : 7.f;
 constexpr int kItems = 4;          // work items handed out ahead
 // Least work of a CTA, in key tiles: few requests are spread wide, but not so that most
 // of a CTA's time is its start (one token: 777 rows 12.3 us with 4, 11.5 with 2, 11.2 with 1;
@@ -383,6 +389,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Logarithm of a row's sum of exponentials, from its maximum and its sum.
+template <bool BF16>
+__device__ __forceinline__ float lse_of(float m, float l) {
+  constexpr float kUnlift = BF16 ? 1.f : 1.f / 128.f;
+  static_assert(kLift<BF16> == (BF16 ? 0.f : 7.f));
+  return l == 0.f ? -INFINITY : (m + log2f(l * kUnlift)) * 0.6931471805599453f;
 }
 __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   f2 d;
@@ -851,7 +864,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
               tmem_st_16(to + c, o);
             }
           }
-          const float base = !live ? -INFINITY : m == -INFINITY ? 0.f : -m;  // (no row: P = 0)
+          const float base = !live ? -INFINITY : m == -INFINITY ? 0.f : kLift<BF16> - m;  // (no row: P = 0)
           const f2 base2 = f2_make(base, base);
           f2 sums[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
@@ -957,7 +970,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             part[kTile * D + row] = m;
             part[kTile * D + kTile + row] = l;
           } else if (p.lse) {
-            p.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            p.lse[out_row] = lse_of<BF16>(m, l);
           }
         }
       }
@@ -1055,7 +1068,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join(const TreeAttnArg
       *reinterpret_cast<uint4*>(p.out + r * D + chunk * 8) =
           make_uint4(pack_pair<BF16>(j.v[0] * inv, j.v[1] * inv), pack_pair<BF16>(j.v[2] * inv, j.v[3] * inv),
                      pack_pair<BF16>(j.v[4] * inv, j.v[5] * inv), pack_pair<BF16>(j.v[6] * inv, j.v[7] * inv));
-      if (p.lse && chunk == 0) p.lse[r] = j.l == 0.f ? -INFINITY : (j.m + log2f(j.l)) * 0.6931471805599453f;
+      if (p.lse && chunk == 0) p.lse[r] = lse_of<BF16>(j.m, j.l);
     }
   }
 }

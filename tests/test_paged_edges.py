@@ -1,5 +1,5 @@
 """Edges of the paged operators: requests that outgrow their row of the table, the
-largest lengths, and tokens of no request."""
+largest lengths, tokens of no request, and small fp16 probabilities."""
 from __future__ import annotations
 
 import numpy as np
@@ -104,4 +104,38 @@ def test_attention_rows_in_front_of_the_first_request(first, end):
     assert (got[cu[2]:] == 0).all() and (lse[cu[2]:] == -float("inf")).all()
     want = ng.tree_attention(q[first:cu[2]], k, v, table, ints([50, 20]), ints([0, 4, 9]))
     assert torch.equal(got[first:cu[2]], want)
+    tp.assert_clean()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tall_at", [0, 40, 63])
+@pytest.mark.parametrize("new", [1, 5])
+def test_attention_small_fp16_probabilities(dim, tall_at, new):
+    """Keys whose probability is 2^-25.5 of the largest still count in the output.
+
+    fp16 has no value below 2^-24 of its own unit, but the kernel's probabilities reach up to
+    2^15, so none above 2^-33 of the row's largest is lost: each is off by at most 2^-32."""
+    page, kv, big = 16, 64 + new - 1, 1024.0
+    k, v = ng.paged_cache(8, page, 1, dim)
+    table = ints([range(8)])
+    q = torch.zeros(new, 2, dim, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1
+    rows = torch.arange(kv, device="cuda")
+    height = torch.full((kv,), -25.5, device="cuda")
+    height[tall_at] = 0
+    k[rows // page, rows % page, 0, 0] = height.half()  # exact; scores in base 2
+    value = torch.full((kv,), big, device="cuda")
+    value[tall_at] = 0
+    v[rows // page, rows % page, 0] = value.half()[:, None]
+    scale = float(np.log(2.0))
+    got, lse = ng.tree_attention(q, k, v, table, ints([kv]), ints([0, new]), scale=scale, return_lse=True)
+    for i in range(new):
+        seen = kv - new + i + 1
+        p = torch.exp2(height[:seen].double())
+        want = (p * value[:seen].double()).sum() / p.sum()
+        # rounding of the result and of P, fp32 scores (25.5 * 2^-24 of a unit), and 2^-32 for each key
+        tol = want * (2 * 2.0**-11 + 1e-5) + seen * 2.0**-32 * big + 2.0**-25
+        assert want > 4 * tol  # all of it would be missed otherwise
+        assert ((got[i].double() - want).abs() <= tol).all()
+        assert ((lse[i].double() - p.sum().log()).abs() <= 1e-6).all()
     tp.assert_clean()
