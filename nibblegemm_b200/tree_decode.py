@@ -35,7 +35,8 @@ class TreeStep(NamedTuple):
 
 
 class TreeDecoder:
-    """Serves up to ``requests`` sequences from a pool of ``num_pages`` pages.
+    """Serves up to ``requests`` sequences at a time from a pool of ``num_pages`` pages;
+    ``step`` runs their new tokens, ``release`` ends some of them.
 
     ``model`` supplies weights and configuration (its own contiguous caches are not
     used: build it with a small ``max_ctx``).  ``q_norm`` / ``k_norm`` ([layers] lists of
@@ -116,6 +117,24 @@ class TreeDecoder:
         self.held.copy_(plan.held)
         self.cursor += plan.taken
         return TreeStep(out, accepted, path, next_tokens, granted)
+
+    def release(self, done: torch.Tensor) -> None:
+        """End the requests where ``done`` (bool [requests], on the GPU) is set: their pages go
+        back to the pool and their places can take new requests.  Nothing is read back."""
+        if done.shape != self.cached.shape or done.dtype != torch.bool or done.device != self.cached.device:
+            raise ValueError("done must be a bool [requests] tensor on the decoder's device")
+        n = self.free_pages.numel()
+        mine = (done[:, None] & (torch.arange(self.table.size(1), device=done.device) < self.held[:, None])).flatten()
+        back = mine.sum()
+        # The entries in front of the cursor stand for pages in use, so that is where the
+        # pages go; entry n is for the rest of the table.
+        at = torch.where(mine, self.cursor - back + mine.cumsum(0) - 1, n)
+        pages = torch.cat([self.free_pages, self.free_pages[:1]]).scatter_(0, at, self.table.flatten())
+        self.free_pages.copy_(pages[:n])
+        self.cursor -= back
+        for x in (self.cached, self.held):
+            x.masked_fill_(done, 0)
+        self.table.masked_fill_(done[:, None], -1)
 
     def _head(self, xn: torch.Tensor) -> torch.Tensor:
         """The model's token after every row of the normed hidden state."""
