@@ -139,3 +139,20 @@ def test_attention_small_fp16_probabilities(dim, tall_at, new):
         assert ((got[i].double() - want).abs() <= tol).all()
         assert ((lse[i].double() - p.sum().log()).abs() <= 1e-6).all()
     tp.assert_clean()
+
+
+@pytest.mark.parametrize("dtype", tp.DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_lse_of_equal_scores(dtype, dim):
+    """With queries of zeros every visible key weighs the same: lse is the logarithm of their number."""
+    rng = np.random.default_rng(dim)
+    new, kv = [3, 1, 70, 2], [700, 9001, 300, 2]
+    k, v, table = tp.build_pages(rng, kv, 16, 2, dim, dtype, False)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = torch.zeros(int(cu[-1]), 4, dim, device="cuda", dtype=dtype)
+    got, lse = ng.tree_attention(q, k, v, table, ints(kv), ints(cu), return_lse=True)
+    tp.check_attn(got, lse, tp.attn_reference(q, k, v, table, kv, cu, None, dim**-0.5), dtype)
+    seen = np.concatenate([np.arange(L - n + 1, L + 1) for n, L in zip(new, kv)])
+    want = torch.as_tensor(np.log(seen), device="cuda")[:, None]
+    assert ((lse.double() - want).abs() <= 2e-7 * want + 5e-7).all()  # sums of ones are exact; log2 and one product
+    tp.assert_clean()
