@@ -398,7 +398,8 @@ int ng_embed_tokens(const long long* tokens, long long* keys, long long* tokens_
  *     in each of `layers` caches (stride_layer apart) row before + i becomes row
  *     before + path[i], before = kv_lens[b] - n.  accepted [B], path [B, max_path] (-1 beyond),
  *     bonus [B] = next at the path's end (-1 without tokens), kv_out [B] =
- *     before + accepted (a request without tokens keeps kv_lens). */
+ *     before + accepted (a request without tokens keeps kv_lens; one that was not granted
+ *     has the 0 of its plan here too, and its cached length is what it was). */
 int ng_paged_plan(const int* cached, const int* new_lens, const int* held, int* block_table,
                   long long table_stride, int table_width, const int* free_pages, int num_free,
                   const int* cursor, const int* parents, int B, int num_tokens, int page_size,

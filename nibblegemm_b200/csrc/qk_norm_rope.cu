@@ -20,8 +20,8 @@
 // Bound: HBM for many tokens.  Four rows are loaded ahead (with one, the loads
 // of a warp were exposed one after another: 56 us where four take 40; two, three and six
 // are slower).  128 registers a thread, 16 warps an SM (20 of 96: 2000 tokens of 48 rows
-// 14.0 us, not 11.7).  8192 tokens of 48 rows of 128, bf16, on a B200: 38.9 us, 5.2 TB/s;
-// 976 tokens of 80 rows 10.7 us, one round of loads after another; 4 tokens 2.2 us, the
+// 14.0 us, not 11.7).  8192 tokens of 48 rows of 128, bf16, on a B200: 38.4 us, 5.2 TB/s;
+// 976 tokens of 80 rows 9.5 us, one round of loads after another; 4 tokens 2.3 us, the
 // launch.
 #include <algorithm>
 

@@ -44,14 +44,16 @@
 // rows that do see them.  Only tiles that hold such keys pay for this.
 //
 // Bound: HBM for single tokens, where every K and V row is used by G rows only; the tensor
-// core for many rows, at 12 products a tile (Q K^T 8 of 61 cycles, as 64 keys re-read
-// all of Q; P V 4 of 65): 825 cycles a tile of 128 x 64 on an SM, 748 of them its products'.
-// 32 query heads, 8 KV heads of 128, bf16, on a B200:
-//   64 single tokens, up to 8192 rows   205 us  6.4 TB/s
-//   32 trees of up to 64, 4096 rows     102 us  3.5 TB/s, 625 TFLOP/s
-//   3 x up to 2048 tokens, 4096 rows    343 us  1025 TFLOP/s
-//   1000 single tokens, up to 500 rows  213 us  5.9 TB/s
-//   1 token, 777 rows (fp16)           10.8 us
+// core and the softmax for many rows.  The twelve products of a tile (Q K^T 8 of 61 cycles, as 64 keys
+// re-read all of Q; P V 4 of 65) take 748 cycles alone, 512 of them arithmetic; a tile of 128 x 64
+// takes an SM 1011 cycles (prompts below, by their time and clock).
+// 32 query heads, 8 KV heads of 128, bf16, on a B200, calls of a CUDA graph of a few milliseconds,
+// with the mean SM clock (of 1965 MHz; the power limit sets it), and after a second of them:
+//   64 single tokens, up to 8192 rows   207 us at 1831 MHz  6.4 TB/s                213 us
+//   32 trees of up to 64, 4096 rows     107 us at 1660 MHz  3.4 TB/s, 600 TFLOP/s   124 us
+//   3 x up to 2048 tokens, 4096 rows    349 us at 1685 MHz  1010 TFLOP/s            400 us
+//   1000 single tokens, up to 500 rows  214 us at 1834 MHz  5.8 TB/s                237 us
+//   1 token, 777 rows (fp16)           10.5 us
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -76,11 +78,11 @@ template <bool BF16>
 constexpr float kLift = BF16 ? 0.f : 7.f;
 constexpr int kItems = 4;          // work items handed out ahead
 // Least work of a CTA, in key tiles: few requests are spread wide, but not so that most
-// of a CTA's time is its start (one token: 777 rows 12.3 us with 4, 11.5 with 2, 11.2 with 1;
-// 4000 rows 13.9, 13.0 and 14.9; a tree of 60 over 2000 rows 24.6, 21.7 and 21.6).
+// of a CTA's time is its start (one token over 777 rows: 12.0 us with 4, 10.8 with 2, 11.1 with 1;
+// over 4000 rows 13.9, 13.4 and 15.4; a tree of 60 over 2000 rows 25.7, 22.4 and 22.4).
 constexpr int kMinUnits = 2;
-// What an item costs beside its key tiles, in key tiles (32 trees: 108 us with 1, 104.8 with 4,
-// 104.2 with 6; 1000 short contexts 280, 275 and 276).
+// What an item costs beside its key tiles, in key tiles (32 trees: 110.5 us with 1, 107.3 with 4,
+// 106.9 with 6; 1000 short contexts 213, 218 and 221; one token over 100 rows 10.6, 9.1 and 9.1).
 constexpr int kItemUnits = 4;
 
 // A work item as one CTA sees it.
@@ -120,7 +122,7 @@ struct alignas(16) Meta {
 // wherever five dimensions can name them: 64 values, 8 rows, halves, groups, and a last
 // one that goes through heads and pages alike or has the heads joined to the halves.
 // Boxes of 16 rows x 128 bytes, one for each half, were issued too slowly: prompts of
-// 16-row pages took 384 us instead of 343.  Strides that no such view fits are read in
+// 16-row pages took 385 us where whole rows took 350, all else alike.  Strides that no such view fits are read in
 // boxes of 8 rows and one half (split).
 struct BoxPlan {
   int split;
@@ -1201,7 +1203,7 @@ extern "C" int ng_tree_attn(const void* q, long long q_stride_token, long long q
                        static_cast<Meta*>(workspace), dev.err};
   auto st = static_cast<cudaStream_t>(stream);
   // As many tokens as one tile holds: no request has two tiles, and the kernel without the
-  // line of pairs starts sooner (one token, 777 rows: 12.3 us instead of 12.8).
+  // line of pairs starts sooner (one token, 777 rows: 10.8 us instead of 11.6).
   auto launch = [&](auto bf16, auto dim) {
     return T <= a.tok_tile ? launch_tree_attn<bf16.value, dim.value, false>(mk, mv, mtile, mtoken, a, dev, st)
                            : launch_tree_attn<bf16.value, dim.value, true>(mk, mv, mtile, mtoken, a, dev, st);

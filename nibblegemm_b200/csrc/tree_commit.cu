@@ -17,8 +17,8 @@
 // memory: two rounds of global loads instead of two for every node of the path.
 // Trees of more nodes than fit there are walked with a ballot over the children.
 //
-// Bound: latency for few trees (4 of 32 nodes, 32 layers: 3.8 us on a B200), then HBM (64
-// of them: 7.4 us; the 50 MB that move would take 7.7 us from HBM, part of them is in L2).
+// Bound: latency for few trees (4 of 32 nodes, 32 layers: 3.6 us on a B200), then HBM (64
+// of 64 nodes: 7.1 us; 31 MB move, 1.84 rows a tree, which alone would take 4.7 us).
 #include <algorithm>
 
 #include "paged_common.cuh"

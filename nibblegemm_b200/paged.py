@@ -48,7 +48,7 @@ class TreeCommit(NamedTuple):
     accepted: torch.Tensor  # int32 [requests]: kept nodes, the root among them
     path: torch.Tensor  # int32 [requests, max_path]: their places in the tree, -1 beyond
     bonus: torch.Tensor  # int64 [requests]: the model's token after the last kept node
-    kv_lens: torch.Tensor  # int32 [requests]: cached tokens after the step
+    kv_lens: torch.Tensor  # int32 [requests]: cached tokens after the step; 0 where the plan granted nothing
 
 
 def _binding():
@@ -144,7 +144,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     chains, prompts and single tokens need none.  A token that sees nothing, or is no
     request's, gives zeros.  ``scale`` defaults to 1 / sqrt(D).  Returns out like q, and with
     ``return_lse`` also the fp32 [tokens, q_heads] logarithm of the sum of
-    exponentials (-inf where nothing is seen).  D 64 or 128.
+    exponentials (-inf where nothing is seen).  D 64 or 128.  Scores, sums and the output's
+    accumulation are fp32; the probabilities are rounded to the type of ``q`` for the product with V.
 
     Scratch memory (79 MB) is kept for each stream; a call that is captured takes it from its
     graph's own memory, so graphs may be replayed at the same time."""
@@ -163,7 +164,9 @@ def tree_commit(draft: torch.Tensor, parents: torch.Tensor, next_tokens: torch.T
     ``draft`` token (int64 [tokens]) is the model's ``next_tokens`` at its parent, for at most
     ``max_path`` nodes.  The kept nodes' rows of every layer (``k_cache`` / ``v_cache`` with or without a
     leading layer dimension, in place) move behind the rows that were there
-    before the tree.  ``kv_lens`` and ``cu_new`` are the step's (:class:`PagedPlan`)."""
+    before the tree.  ``kv_lens`` and ``cu_new`` are the step's (:class:`PagedPlan`).  A request
+    that was not granted has ``kv_lens`` 0 there and in the result: its cached tokens are what
+    they were (``cached += accepted`` is right for every request)."""
     *out, status = _binding().tree_commit(draft, parents, next_tokens, cu_new, kv_lens, block_table, k_cache,
                                           v_cache, max_path)
     _done(status, "tree_commit")

@@ -2,8 +2,8 @@
 KV cache: the operators of ``paged.py`` put together as a server uses them.
 
 ``TreeDecoder.step`` takes the new tokens of all requests, of any mix of lengths:
-prompts or single tokens (chains), or drafted trees whose node 0 is the last known
-token.  It plans the step on the GPU, runs the layers (the projections are the
+either prompts and single tokens (chains), or drafted trees whose node 0 is the last known
+token; a step is all of the one or all of the other.  It plans the step on the GPU, runs the layers (the projections are the
 W4A16 GEMV / GEMM), takes the model's token at every node, and keeps the drafted
 path that the model agrees with.  Nothing is read back to the host: contexts, page
 tables and the free list live on the GPU.
@@ -65,7 +65,8 @@ class TreeDecoder:
         ``tokens`` (int64 [total]) lie request behind request.  Without ``parents`` they are
         prompts or single tokens and all are kept.  With ``parents`` (int32 [total], see
         :func:`paged_plan`) they are trees of at most ``max_tree`` nodes, of which the
-        agreed path of at most ``max_path`` is kept."""
+        agreed path of at most ``max_path`` is kept (so a prompt does not go with them: it would be
+        kept as far as the model happens to agree with it).  The head runs on every new token."""
         m, cfg = self.model, self.model.cfg
         if tokens.dim() != 1 or tokens.dtype != torch.int64 or not tokens.is_cuda:
             raise ValueError("tokens must be a 1-D int64 CUDA tensor")
