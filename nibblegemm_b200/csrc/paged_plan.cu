@@ -244,7 +244,7 @@ extern "C" int ng_paged_plan(const int* cached, const int* new_lens, const int* 
     return NG_ERR_NULL_POINTER;
   if (num_tokens > 0 && (!slots || !positions)) return NG_ERR_NULL_POINTER;
   if (num_free > 0 && !free_pages) return NG_ERR_NULL_POINTER;
-  if (mask_words > 0 && (!parents || (num_tokens > 0 && !mask))) return NG_ERR_NULL_POINTER;
+  if (mask_words > 0 && num_tokens > 0 && (!parents || !mask)) return NG_ERR_NULL_POINTER;
   if (B < 1 || B > kPlanMaxBatch || num_tokens < 0 || num_tokens > (1 << 30) || num_free < 0 ||
       table_width < 1 || table_stride < table_width || !page_size_ok(page_size))
     return NG_ERR_BAD_SHAPE;

@@ -76,6 +76,19 @@ def test_plan_of_the_largest_lengths(cached, new, page):
     assert ng.extension().device_status() == (10 if over else 0)
 
 
+@pytest.mark.parametrize("words", [0, 2])
+def test_plan_without_tokens(words):
+    """A step of trees in which no request has a token."""
+    tab = ints([[3, -1], [5, 6]])
+    p = ng.paged_plan(ints([7, 20]), ints([0, 0]), ints([1, 2]), tab, ints([8]), page_size=16, num_tokens=0,
+                      parents=ints([]), mask_words=words)
+    assert p.cu_new.tolist() == [0, 0, 0] and p.kv_lens.tolist() == [7, 20] and p.held.tolist() == [1, 2]
+    assert p.taken.item() == 0 and p.slots.shape == (0,) and p.positions.shape == (0,)
+    assert (p.mask is None) if words == 0 else (p.mask.shape == (0, words))
+    assert tab.tolist() == [[3, -1], [5, 6]]
+    tp.assert_clean()
+
+
 # --------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_without_requests(dim):
