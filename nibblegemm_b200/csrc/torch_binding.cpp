@@ -265,6 +265,12 @@ std::tuple<std::vector<std::optional<torch::Tensor>>, int64_t> paged_plan(
        held_out = slices.take({B}, torch::kInt), taken = slices.take({1}, torch::kInt);
   std::optional<torch::Tensor> mask;
   if (mask_words > 0) mask = slices.take({num_tokens, mask_words}, torch::kLong);
+  if (B == 0) {  // all tokens are rows past the last request's
+    for (auto* t : {&cu, &positions, &taken}) t->zero_();
+    slots.fill_(-1);
+    if (mask) mask->zero_();
+    return {{cu, slots, positions, kv, held_out, taken, mask}, 0};
+  }
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   const int st = ng_paged_plan(
       cached.data_ptr<int>(), fresh.data_ptr<int>(), held.data_ptr<int>(), table.data_ptr<int>(), stride,

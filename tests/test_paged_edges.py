@@ -89,6 +89,17 @@ def test_plan_without_tokens(words):
     tp.assert_clean()
 
 
+@pytest.mark.parametrize("tokens", [0, 4])
+@pytest.mark.parametrize("words", [0, 1])
+def test_plan_without_requests(tokens, words):
+    p = ng.paged_plan(ints([]), ints([]), ints([]), torch.zeros(0, 3, dtype=torch.int32, device="cuda"), ints([1, 2]),
+                      page_size=16, num_tokens=tokens, parents=ints([-1] * tokens) if words else None, mask_words=words)
+    assert p.cu_new.tolist() == [0] and p.kv_lens.shape == (0,) and p.held.shape == (0,) and p.taken.tolist() == [0]
+    assert p.slots.tolist() == [-1] * tokens and p.positions.tolist() == [0] * tokens
+    assert (p.mask is None) if words == 0 else p.mask.tolist() == [[0]] * tokens
+    tp.assert_clean()
+
+
 # --------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_without_requests(dim):
