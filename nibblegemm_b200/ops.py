@@ -128,22 +128,27 @@ class _Extension:
         self._gws = {}  # (device index, stream handle) -> zero-initialised GEMM split-K workspace
         self._outgrown = []  # earlier ones: a captured graph may hold their addresses
 
+    def _cached(self, cache: dict, need: int, least: int, device: torch.device, stream: int) -> torch.Tensor:
+        """The buffer of (device, stream), as the binding keeps it, for the route without it."""
+        ws = cache.get((device.index, stream))
+        have = 0 if ws is None else ws.numel()
+        if ws is not None and have >= need:
+            return ws
+        new = torch.zeros(max(need, 2 * have, least), dtype=torch.uint8, device=device)
+        if torch.cuda.is_current_stream_capturing():
+            return new  # the graph's own: it is filled at replays only, so no later call may find it
+        if ws is not None:
+            self._outgrown.append(ws)
+        cache[(device.index, stream)] = new
+        return new
+
     def gemm_workspace(self, M: int, N: int, device: torch.device, stream: int) -> torch.Tensor:
         """The prefill-GEMM split-K workspace for (device, stream), grown on demand
         (zero-filled once; every call leaves its per-tile counters at zero)."""
         need = self.lib.ng_gemm_workspace_bytes(M, N)
         if self.binding is not None:
             return self.binding.workspace(device.index, stream, 1, need)
-        key = (device.index, stream)
-        ws = self._gws.get(key)
-        if ws is None or ws.numel() < need:
-            have = 0
-            if ws is not None:
-                self._outgrown.append(ws)
-                have = ws.numel()
-            ws = torch.zeros(max(need, 2 * have, 1 << 20), dtype=torch.uint8, device=device)
-            self._gws[key] = ws
-        return ws
+        return self._cached(self._gws, need, 1 << 20, device, stream)
 
     def workspace(self, N: int, device: torch.device, stream: int) -> torch.Tensor:
         """The decode-GEMV workspace for (device, stream), grown on demand.
@@ -155,16 +160,7 @@ class _Extension:
         need = self.lib.ng_gemv_workspace_bytes(1, N)
         if self.binding is not None:
             return self.binding.workspace(device.index, stream, 0, need)
-        key = (device.index, stream)
-        ws = self._ws.get(key)
-        if ws is None or ws.numel() < need:
-            have = 0
-            if ws is not None:
-                self._outgrown.append(ws)
-                have = ws.numel()
-            ws = torch.zeros(max(need, 2 * have, 4 << 20), dtype=torch.uint8, device=device)
-            self._ws[key] = ws
-        return ws
+        return self._cached(self._ws, need, 4 << 20, device, stream)
 
     def dequant_w4(self, Wq: torch.Tensor, S: torch.Tensor, group_size: int, fast: bool = True,
                    out_dtype: torch.dtype = torch.float16) -> torch.Tensor:

@@ -140,3 +140,36 @@ def test_graphs_of_one_stream_replayed_at_the_same_time(dim):
         for out, w in zip(outs, want):
             assert torch.equal(out, w)
     tp.assert_clean()
+
+
+def test_the_route_without_the_binding():
+    """Its buffers are kept in Python, under the same rules."""
+    torch.manual_seed(0)
+    K, N = 512, 1024
+    ext, qw = ng.extension(), ng.quantize(torch.randn(K, N)).to("cuda")
+    x, many = (torch.randn(m, K, device="cuda").half() for m in (1, 128))
+    plain = type(ext)()
+    plain.binding = None
+    calls = (lambda e: e.gemv_w4a16(x, qw.qweight, qw.scales, 128)), (lambda e: e.gemm_w4a16(many, qw.qweight, qw.scales, 128))
+    want = [f(ext) for f in calls]
+    torch.cuda.synchronize()
+    s, graph = fresh_stream(), torch.cuda.CUDAGraph()
+    key = (torch.cuda.current_device(), s.cuda_stream)
+    with torch.cuda.graph(graph, stream=s):
+        got = [f(plain) for f in calls]
+    assert key not in plain._ws and key not in plain._gws
+    with torch.cuda.stream(s):
+        for y, w in zip([f(plain) for f in calls], want):
+            assert torch.equal(y, w)
+        graph.replay()
+    torch.cuda.synchronize()
+    for y, w in zip(got, want):
+        assert torch.equal(y, w)
+    with torch.cuda.stream(s):
+        old = plain._ws[key].data_ptr()
+        size = plain._ws[key].numel()
+        grown = plain._cached(plain._ws, size + 1, 1, x.device, s.cuda_stream)
+        assert grown.data_ptr() != old and plain._ws[key] is grown
+        others = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
+        assert all(y.data_ptr() != old for y in others)
+    tp.assert_clean()
