@@ -89,7 +89,9 @@ torch::Tensor workspace(const torch::Device& dev, cudaStream_t stream, int kind,
   const size_t have = all.empty() ? 0 : static_cast<size_t>(all.back().numel());
   if (have >= std::max<size_t>(need, 1)) return all.back();
   const c10::cuda::CUDAGuard guard(dev);
-  const size_t least = kind == kAttentionWorkspace ? ng_tree_attn_workspace_bytes(128) : kind == kGemvWorkspace ? 4u << 20 : 1u << 20;
+  const size_t least = kind == kAttentionWorkspace ? ng_tree_attn_workspace_bytes(128)
+                       : kind == kGemvWorkspace    ? 4u << 20
+                                                   : 1u << 20;
   const auto bytes = static_cast<int64_t>(std::max({need, 2 * have, least}));
   const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
   auto make = [&] { return kind == kAttentionWorkspace ? torch::empty({bytes}, options) : torch::zeros({bytes}, options); };

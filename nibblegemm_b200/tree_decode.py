@@ -2,11 +2,11 @@
 KV cache: the operators of ``paged.py`` put together as a server uses them.
 
 ``TreeDecoder.step`` takes the new tokens of all requests, of any mix of lengths:
-either prompts and single tokens (chains), or drafted trees whose node 0 is the last known
-token; a step is all of the one or all of the other.  It plans the step on the GPU, runs the layers (the projections are the
-W4A16 GEMV / GEMM), takes the model's token at every node, and keeps the drafted
-path that the model agrees with.  Nothing is read back to the host: contexts, page
-tables and the free list live on the GPU.
+either prompts and single tokens (chains), or drafted trees whose node 0 is the last
+known token; a step is all of the one or all of the other.  It plans the step on the GPU,
+runs the layers (the projections are the W4A16 GEMV / GEMM), takes the model's token at
+every node, and keeps the drafted path that the model agrees with.  Nothing is read back
+to the host: contexts, page tables and the free list live on the GPU.
 
 The reference (arvindcr4/nibblegemm) has no counterpart; its decode step is
 projections only (``bench/bench_model.py:57-86``).
